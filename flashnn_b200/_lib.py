@@ -48,6 +48,22 @@ SIGNATURES = {
                                           _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int,
                                           _c.c_int, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "fnn_fused_moe_a16w4_workspace_bytes": (_c.c_size_t, [_c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int]),
+    "fnn_gemm_a8w8_epilogue": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int,
+                                          _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_int, _c.c_int, _c.c_int,
+                                          _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64,
+                                          _c.c_int64, _c.c_void_p]),
+    "fnn_fused_moe_a8w8_gated": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int64,
+                                            _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_int, _c.c_int,
+                                            _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_int,
+                                            _c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "fnn_moe_route": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int, _c.c_int,
+                                 _c.c_int, _c.c_int, _c.c_int, _c.c_float, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "fnn_moe_sort": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_int64,
+                                _c.c_void_p, _c.c_void_p, _c.c_void_p]),
+    "fnn_moe_sort_slots": (_c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int]),
+    "fnn_moe_combine": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64,
+                                   _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p,
+                                   _c.c_int64, _c.c_void_p]),
     "fnn_set_option": (_c.c_int, [_c.c_int, _c.c_int]),
     "fnn_get_option": (_c.c_int, [_c.c_int]),
     "fnn_rms_norm_dquant": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_int,
@@ -101,6 +117,11 @@ def check(status: int):
         raise FlashNNError(status, f"{l.fnn_status_string(status).decode()}: "
                                    f"{l.fnn_last_error_string().decode()}")
 
+
+# fnn_activation, fnn_moe_scoring and fnn_moe_group_score by name
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "sigmoid": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
 
 OPT_STATIC_WEIGHTS = 1
 OPT_TEST_STALL_US = 2  # test hook, see include/flashnn_b200.h

@@ -23,6 +23,7 @@
 
 #include "a8w8_plan.h"
 #include "common.cuh"
+#include "epilogue.cuh"
 
 namespace fnn {
 namespace {
@@ -70,13 +71,14 @@ struct A8W8Params {
 // bounds that is the bytes a CTA keeps in flight, so their stages carry only the rows of A that exist and there are
 // more of them.  The tensor core still reads 128 rows from the A base (what lies behind the real rows belongs to the
 // following buffers; the accumulator rows it produces are never stored), so the last stage is followed by padding.
-template <int BN, int STAGES, int AROWS = kBM> struct SmemLayout {
+template <int BN, int STAGES, int AROWS = kBM, bool BIAS = false> struct SmemLayout {
+  static constexpr int kColWords = (BIAS ? 2 : 1) * BN;  // per epilogue warp: column scales, then (fused epilogue) biases
   static constexpr int kABytes = AROWS * kBK;
   static constexpr int kBBytes = BN * kBK;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kTailPad = (kBM * kBK > kStageBytes) ? kBM * kBK - kStageBytes : 0;
-  static constexpr int kColScaleOff = STAGES * kStageBytes + kTailPad;  // [4][BN] float
-  static constexpr int kBarOff = kColScaleOff + 4 * BN * 4;          // barriers
+  static constexpr int kColScaleOff = STAGES * kStageBytes + kTailPad;  // [4][kColWords] float
+  static constexpr int kBarOff = kColScaleOff + 4 * kColWords * 4;   // barriers
   static constexpr int kNumBars = 2 * STAGES + 4 + 1;                // full, empty, tmem full/empty x2, drain
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kAbortOff = kTmemSlotOff + 8;
@@ -189,11 +191,68 @@ __device__ __forceinline__ void store_chunk_moe(const uint32_t (&r)[32], int64_t
   }
 }
 
-template <typename OutT, int BN, int STAGES, bool MOE, int AROWS>
+// Column scales (and biases) of a tile's accumulator columns [j0, j0 + count) -> this warp's shared copy, as fp32.
+// Accumulator column j is weight row n0 + j; with a gate the tile's upper half of the columns are rows N + n0 + j.
+template <int BN, class FX>
+__device__ __forceinline__ void stage_columns(float* cs, int j0, int count, int n0, int64_t col_base, int lane, const A8W8Params& p,
+                                              const FX& fx) {
+  for (int j = j0 + lane; j < j0 + count; j += 32) {
+    if constexpr (FX::kOn) {
+      constexpr int OW = FX::kGated ? BN / 2 : BN;
+      const int n = n0 + (j < OW ? j : j - OW);
+      const int64_t at = col_base + n + (j < OW ? 0 : p.N);
+      cs[j] = n < p.N ? load_as_f32(p.alpha_col, p.col_dtype, at) : 0.f;
+      cs[BN + j] = (n < p.N && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, at) : 0.f;
+    } else {
+      cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
+    }
+  }
+}
+
+// Fused epilogue of 32 output columns of one row up to (not including) the residual: `r` are their sums and, with a
+// gate, `u` those of the rows that the activated value multiplies; cs is this warp's staged scales and biases, c32 the
+// first output column within the tile.
+template <int BN, class FX>
+__device__ __forceinline__ void fused_chunk(const uint32_t (&r)[32], const uint32_t (&u)[32], float rs, const float* cs, int c32,
+                                            bool same16, const A8W8Params& p, const FX& fx, float (&v)[32]) {
+  scale_chunk(r, rs, cs + c32, same16, p, v);
+  add_bias32(cs + BN + c32, v);
+  activate_n(v, fx.act);
+  if constexpr (FX::kGated) {
+    float w[32];
+    scale_chunk(u, rs, cs + BN / 2 + c32, same16, p, w);
+    add_bias32(cs + BN + BN / 2 + c32, w);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= w[j];
+  }
+}
+
+// 32 finished values of one output row
+template <typename OutT>
+__device__ __forceinline__ void store_values(const float (&v)[32], int64_t row, int col0, const A8W8Params& p, bool vec_ok) {
+  OutT* orow = reinterpret_cast<OutT*>(p.out) + row * p.ldo + col0;
+  if (col0 + 32 <= p.N && vec_ok) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8)
+      *reinterpret_cast<uint4*>(orow + j) =
+          make_uint4(pack2<OutT>(v[j], v[j + 1]), pack2<OutT>(v[j + 2], v[j + 3]),
+                     pack2<OutT>(v[j + 4], v[j + 5]), pack2<OutT>(v[j + 6], v[j + 7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < p.N) orow[j] = from_f32<OutT>(v[j]);
+  }
+}
+
+// FX: NoEpilogue, or the fused epilogue (epilogue.cuh).  With a gate a tile has BN / 2 output columns: its BN accumulator
+// columns are BN / 2 weight rows of each half.
+template <typename OutT, int BN, int STAGES, bool MOE, int AROWS, class FX = NoEpilogue>
 __global__ void __launch_bounds__(kThreads, 1)
 a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                 const A8W8Params p) {
-  using L = SmemLayout<BN, STAGES, AROWS>;
+                 const A8W8Params p, const FX fx) {
+  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn>;
+  constexpr int OW = FX::kGated ? BN / 2 : BN;  // output columns of a tile
+  static_assert(OW % 32 == 0, "whole chunks of 32 output columns");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* col_scale_smem = reinterpret_cast<float*>(smem + L::kColScaleOff);
@@ -250,7 +309,9 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       tile_coords(t, p.tiles_m, p.tiles_n, mb, nb);
       if (MOE && mb * tile_rows >= rows_in_use) continue;
       // fused MoE: the tile's weights are rows [e * N + nb * BN, ...) of the expert stack
-      const int b_row = nb * BN + (MOE ? __ldg(p.expert_ids + (mb * tile_rows) / p.block_m) * p.N : 0);
+      int weight_rows = p.N;  // of one expert
+      if constexpr (FX::kOn) weight_rows = fx.rows;
+      const int b_row = nb * OW + (MOE ? __ldg(p.expert_ids + (mb * tile_rows) / p.block_m) * weight_rows : 0);
       for (int kb = 0; kb < p.k_blocks; ++kb) {
         ok = mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
@@ -263,6 +324,7 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
           mbar_expect_tx(&full_bar[stage], L::kStageBytes);
           tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * kBK, mb * tile_rows);
           tma_load_2d(sa + L::kABytes, &tmap_b, &full_bar[stage], kb * kBK, b_row);
+          if (FX::kGated) tma_load_2d(sa + L::kABytes + OW * kBK, &tmap_b, &full_bar[stage], kb * kBK, b_row + p.N);
           ++issued;
         }
         __syncwarp();
@@ -339,10 +401,13 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
   } else {
     // -------------------------------- epilogue --------------------------------
     const int quarter = warp & 3;
-    float* cs = col_scale_smem + quarter * BN;  // this warp's private copy
-    const bool same16 = (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
+    float* cs = col_scale_smem + quarter * L::kColWords;  // this warp's private copy
+    // (the expert products take the scales' product in fp32 whatever their dtypes are)
+    const bool same16 = !MOE && (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
     const bool vec_ok = (p.ldo % 8 == 0) && (reinterpret_cast<uintptr_t>(p.out) % 16 == 0);
     const bool acc_vec_ok = p.acc_out && (p.ldacc % 4 == 0) && (reinterpret_cast<uintptr_t>(p.acc_out) % 16 == 0);
+    bool res_vec_ok = false;
+    if constexpr (FX::kOn) res_vec_ok = (fx.ldr % 8 == 0) && (reinterpret_cast<uintptr_t>(fx.residual) % 16 == 0);
     int local = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
@@ -353,17 +418,22 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       const uint32_t acc_phase = (local >> 1) & 1;
       ++local;
       const int row = mb * tile_rows + quarter * 32 + lane;
-      const int n0 = nb * BN;
+      const int n0 = nb * OW;
       // column scales of this tile -> this warp's smem copy (fp32); row scale -> register
-      const int64_t col_base = MOE ? int64_t(__ldg(p.expert_ids + (mb * tile_rows) / p.block_m)) * p.col_stride_e : 0;
-      for (int j = lane; j < BN; j += 32)
-        cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
+      int64_t col_base = 0;
+      bool expert_ok = true;
+      if (MOE) {
+        const int e = __ldg(p.expert_ids + (mb * tile_rows) / p.block_m);
+        if constexpr (FX::kOn) expert_ok = unsigned(e) < unsigned(fx.experts);
+        col_base = expert_ok ? int64_t(e) * p.col_stride_e : 0;
+      }
+      stage_columns<BN>(cs, 0, BN, n0, col_base, lane, p, fx);
       float rs = 0.f, rw = 1.f;
       int64_t out_row = -1;  // fused MoE: the flat (token, choice) index this slot writes, or -1
       if (MOE) {
         if (quarter * 32 + lane < tile_rows) {
           const int flat = __ldg(p.sorted_ids + row);
-          if (flat >= 0 && flat < p.num_valid) {
+          if (flat >= 0 && flat < p.num_valid && expert_ok) {
             out_row = flat;
             rs = load_as_f32(p.alpha_row, p.row_dtype, flat / p.top_k);
             if (p.mul_w) rw = load_as_f32(p.topk_w, p.topk_w_dtype, flat);
@@ -383,11 +453,24 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       tc_fence_after();
       const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + buf * BN;
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t r[32];
+      for (int c = 0; c < OW / 32; ++c) {
+        uint32_t r[32], u[32];
         tmem_ld_32x32(taddr + c * 32, r);
+        if (FX::kGated) tmem_ld_32x32(taddr + OW + c * 32, u);
         tc_wait_ld();
-        if (MOE) {
+        if constexpr (FX::kOn) {
+          const int64_t to = MOE ? out_row : (row < p.M ? row : -1);
+          if (to >= 0 && n0 + c * 32 < p.N) {
+            float v[32];
+            fused_chunk<BN>(r, u, rs, cs, c * 32, same16, p, fx, v);
+            if (!MOE && fx.residual) {
+              uint32_t res[16];
+              load_residual32<OutT>(fx, row, n0 + c * 32, p.M, p.N, res_vec_ok, res);
+              add_residual32<OutT>(res, v);
+            }
+            store_values<OutT>(v, to, n0 + c * 32, p, vec_ok);
+          }
+        } else if (MOE) {
           if (out_row >= 0) store_chunk_moe<OutT>(r, out_row, n0 + c * 32, rs, rw, p.mul_w != 0, cs + c * 32, p, vec_ok);
         } else {
           store_chunk<OutT>(r, row, n0 + c * 32, rs, cs + c * 32, same16, p, vec_ok, acc_vec_ok);
@@ -521,7 +604,8 @@ __device__ __forceinline__ bool flag_wait_bounded(const unsigned long long* f, u
   }
 }
 
-template <int BN, int STAGES, int EPI = 4> struct PairSmem {
+template <int BN, int STAGES, int EPI = 4, bool BIAS = false> struct PairSmem {
+  static constexpr int kColWords = (BIAS ? 2 : 1) * BN;  // per epilogue warp: column scales, then (fused epilogue) biases
   static constexpr int kBN = BN;                        // output columns of a pair tile (a multiple of 32, at most 256)
   static constexpr int kABytes = kBM * kBK;             // this CTA's 128 rows of A
   static constexpr int kBBytes = (kBN / 2) * kBK;       // this CTA's BN / 2 rows of B
@@ -529,8 +613,8 @@ template <int BN, int STAGES, int EPI = 4> struct PairSmem {
   static constexpr int kOutOff = STAGES * kStageBytes;        // [EPI epilogue warps][2][32 rows x 64 B] output staging
   static constexpr int kOutBufs = EPI == 4 ? 2 : 1;           // staging buffers per epilogue warp
   static constexpr int kOutBytes = EPI * kOutBufs * 2048;
-  static constexpr int kColScaleOff = kOutOff + kOutBytes;    // [EPI][kBN] float
-  static constexpr int kBarOff = kColScaleOff + EPI * kBN * 4;
+  static constexpr int kColScaleOff = kOutOff + kOutBytes;    // [EPI][kColWords] float
+  static constexpr int kBarOff = kColScaleOff + EPI * kColWords * 4;
   static constexpr int kNumBars = 2 * STAGES + 4 + 1;
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kAbortOff = kTmemSlotOff + 8;
@@ -542,12 +626,15 @@ template <int BN, int STAGES, int EPI = 4> struct PairSmem {
 // expert picks the weight rows and column scales; the epilogue scatters each slot's row to its (token, choice) index.
 // EPI: epilogue warps per CTA, 4 or 8.  With 8 (the plain mode's default), two warps share a TMEM lane quarter and
 // split a tile's column chunks, and each has one output staging buffer instead of two.
-template <typename OutT, int BN, int STAGES, bool SK, bool MOE = false, int EPI = 4>
+template <typename OutT, int BN, int STAGES, bool SK, bool MOE = false, int EPI = 4, class FX = NoEpilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((2 + EPI) * 32, 1)
 a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                      const __grid_constant__ CUtensorMap tmap_out, const A8W8Params p) {
-  using L = PairSmem<BN, STAGES, EPI>;
-  static_assert(EPI == 4 || (EPI == 8 && !SK && !MOE), "eight epilogue warps exist for the plain mode only");
+                      const __grid_constant__ CUtensorMap tmap_out, const A8W8Params p, const FX fx) {
+  using L = PairSmem<BN, STAGES, EPI, FX::kOn>;
+  static_assert(EPI == 4 || (EPI == 8 && !SK && (!MOE || FX::kOn)), "eight epilogue warps exist for the plain mode only");
+  static_assert(!(SK && FX::kOn), "no K-balanced mode with a fused epilogue");
+  constexpr int OW = FX::kGated ? BN / 2 : BN;  // output columns of a tile
+  static_assert(OW % 32 == 0, "whole chunks of 32 output columns");
   constexpr int kAccStride = 256;  // TMEM columns between the two accumulators (512 are allocated whatever BN is)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -606,7 +693,10 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       int mb, nb;
       tile_coords(w.tile, p.tiles_m, p.tiles_n, mb, nb);
       // fused MoE: the tile's weights are rows [e * N + nb * BN, ...) of the expert stack
-      const int b_row = nb * BN + int(rank) * (BN / 2) + (MOE ? __ldg(p.expert_ids + (mb * 256) / p.block_m) * p.N : 0);
+      // (with a gate the leader's half of the columns are rows inside the activation, the peer's the rows it multiplies)
+      int weight_rows = p.N;  // of one expert
+      if constexpr (FX::kOn) weight_rows = fx.rows;
+      const int b_row = nb * OW + int(rank) * (FX::kGated ? p.N : BN / 2) + (MOE ? __ldg(p.expert_ids + (mb * 256) / p.block_m) * weight_rows : 0);
       for (int kb = w.kb0; kb < w.kb1; ++kb) {
         ok = mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
@@ -690,13 +780,16 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     // -------------------------------- epilogue (both CTAs) --------------------------------
     const int quarter = warp & 3;
     const int ewarp = warp - 2;                  // 0 .. EPI-1
-    constexpr int NC = BN / 32;                  // column chunks of a tile
+    constexpr int NC = OW / 32;                  // column chunks of a tile
     const int c_begin = (EPI == 8 && ewarp >= 4) ? (NC + 1) / 2 : 0;  // with eight warps the second four take the upper chunks
     const int c_end = (EPI == 8 && ewarp < 4) ? (NC + 1) / 2 : NC;
-    float* cs = col_scale_smem + ewarp * BN;  // this warp's private copy
-    const bool same16 = (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
+    float* cs = col_scale_smem + ewarp * L::kColWords;  // this warp's private copy
+    // (the expert products take the scales' product in fp32 whatever their dtypes are)
+    const bool same16 = !MOE && (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
     const bool vec_ok = (p.ldo % 8 == 0) && (reinterpret_cast<uintptr_t>(p.out) % 16 == 0);
     const bool acc_vec_ok = p.acc_out && (p.ldacc % 4 == 0) && (reinterpret_cast<uintptr_t>(p.acc_out) % 16 == 0);
+    bool res_vec_ok = false;
+    if constexpr (FX::kOn) res_vec_ok = (fx.ldr % 8 == 0) && (reinterpret_cast<uintptr_t>(fx.residual) % 16 == 0);
     int local = 0;
     bool ok = true;
     PairWork<SK, MOE> w(p, pair_id, num_pairs);
@@ -719,15 +812,21 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       const int last_h = adds ? ((w.tile + 1) * tail_blocks - 1) / p.sk_tail_units : -1;
       // slot of the piece of this tile that tail-sharing pair h computed: its pieces are of consecutive tiles
       auto slot_of = [&](int h) { return h * p.sk_slots + (w.tile - (h * p.sk_tail_units) / tail_blocks); };
-      const int n0 = nb * BN;
-      const int64_t col_base = MOE ? int64_t(__ldg(p.expert_ids + (mb * 256) / p.block_m)) * p.col_stride_e : 0;
-      for (int j = c_begin * 32 + lane; j < c_end * 32; j += 32)
-        cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
+      const int n0 = nb * OW;
+      int64_t col_base = 0;
+      bool expert_ok = true;
+      if (MOE) {
+        const int e = __ldg(p.expert_ids + (mb * 256) / p.block_m);
+        if constexpr (FX::kOn) expert_ok = unsigned(e) < unsigned(fx.experts);
+        col_base = expert_ok ? int64_t(e) * p.col_stride_e : 0;
+      }
+      stage_columns<BN>(cs, c_begin * 32, (c_end - c_begin) * 32, n0, col_base, lane, p, fx);
+      if (FX::kGated) stage_columns<BN>(cs, OW + c_begin * 32, (c_end - c_begin) * 32, n0, col_base, lane, p, fx);
       float rs = 0.f, rw = 1.f;
       int64_t out_row = -1;  // fused MoE: the flat (token, choice) index this slot writes, or -1
       if (MOE) {
         const int flat = __ldg(p.sorted_ids + row);
-        if (flat >= 0 && flat < p.num_valid) {
+        if (flat >= 0 && flat < p.num_valid && expert_ok) {
           out_row = flat;
           rs = load_as_f32(p.alpha_row, p.row_dtype, flat / p.top_k);
           if (p.mul_w) rw = load_as_f32(p.topk_w, p.topk_w_dtype, flat);
@@ -771,8 +870,13 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       }
 #pragma unroll 1
       for (int c = c_begin; c < c_end; ++c) {
-        uint32_t r[32];
+        uint32_t r[32], u[32];
         tmem_ld_32x32(taddr + c * 32, r);
+        if (FX::kGated) tmem_ld_32x32(taddr + OW + c * 32, u);
+        uint32_t res[16];
+        if constexpr (FX::kOn) {
+          if (!MOE && fx.residual) load_residual32<OutT>(fx, row, n0 + c * 32, p.M, p.N, res_vec_ok, res);
+        }
         uint4 cur[8];
         if (adds) {
 #pragma unroll
@@ -805,7 +909,14 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             }
           }
         }
-        if (MOE) {
+        float v[32];
+        if constexpr (FX::kOn) {
+          fused_chunk<BN>(r, u, rs, cs, c * 32, same16, p, fx, v);
+          if (!MOE && fx.residual) add_residual32<OutT>(res, v);
+        }
+        if (MOE && FX::kOn) {
+          if (out_row >= 0 && n0 + c * 32 < p.N) store_values<OutT>(v, out_row, n0 + c * 32, p, vec_ok);
+        } else if (MOE) {
           if (out_row >= 0) store_chunk_moe<OutT>(r, out_row, n0 + c * 32, rs, rw, p.mul_w != 0, cs + c * 32, p, vec_ok);
         } else if (p.out_tma) {
           // The 32 x 32 block of outputs goes through shared memory and leaves as one TMA store: whole 64-byte row
@@ -813,9 +924,10 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           // piece j of row l sits at piece j ^ ((l >> 1) & 3)), so the 32 lanes' stores spread over all banks; the
           // store leaves out what lies beyond M or N.  Two buffers per warp: before one is written again, the store
           // that read it two chunks ago has finished reading.
-          store_acc_chunk(r, row, n0 + c * 32, p, acc_vec_ok);
-          float v[32];
-          scale_chunk(r, rs, cs + c * 32, same16, p, v);
+          if (!FX::kOn) {
+            store_acc_chunk(r, row, n0 + c * 32, p, acc_vec_ok);
+            scale_chunk(r, rs, cs + c * 32, same16, p, v);
+          }
           if (lane == 0) tma_store_wait_read<L::kOutBufs - 1>();
           __syncwarp();
           uint8_t* buf_out = out_stage + out_buf * 2048;
@@ -831,6 +943,8 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             tma_store_commit();
           }
           if (L::kOutBufs == 2) out_buf ^= 1;
+        } else if (FX::kOn) {
+          if (row < p.M && n0 + c * 32 < p.N) store_values<OutT>(v, row, n0 + c * 32, p, vec_ok);
         } else {
           store_chunk<OutT>(r, row, n0 + c * 32, rs, cs + c * 32, same16, p, vec_ok, acc_vec_ok);
         }
@@ -888,12 +1002,13 @@ inline int make_tmap_i8(CUtensorMap* m, const void* base, int64_t rows, int64_t 
   return make_tmap_2d(m, /*elem_bytes=*/1, base, rows, K, ld, kBK, box_rows, /*swizzle128=*/true);
 }
 
-template <typename OutT, int BN, int STAGES, int AROWS>
-int launch_umma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8Params p, cudaStream_t st) {
-  using L = SmemLayout<BN, STAGES, AROWS>;
+template <typename OutT, int BN, int STAGES, int AROWS, class FX>
+int launch_umma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8Params p, const FX& fx, cudaStream_t st) {
+  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn>;
+  constexpr int OW = FX::kGated ? BN / 2 : BN;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
   static_assert(L::kStageBytes % 1024 == 0 && L::kABytes % 1024 == 0, "tiles must stay 1024-byte aligned");
-  auto kern = a8w8_umma_kernel<OutT, BN, STAGES, false, AROWS>;
+  auto kern = a8w8_umma_kernel<OutT, BN, STAGES, false, AROWS, FX>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];  // per device, so that a failure is reported on every call and not only the first
   int dev = 0;
@@ -905,9 +1020,11 @@ int launch_umma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(a8w8)");
   CUtensorMap ta, tb;
   if (int e = make_tmap_i8(&ta, a, p.M, p.K, lda, AROWS)) return e;
-  if (int e = make_tmap_i8(&tb, b, p.N, p.K, ldb, BN)) return e;
+  int64_t weight_rows = p.N;
+  if constexpr (FX::kOn) weight_rows = fx.rows;
+  if (int e = make_tmap_i8(&tb, b, weight_rows, p.K, ldb, OW)) return e;
   p.tiles_m = (p.M + kBM - 1) / kBM;
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_n = (p.N + OW - 1) / OW;
   p.k_blocks = (p.K + kBK - 1) / kBK;
   if (const int stall_us = opt_test_stall_us()) {  // test hook: make one wait run out quickly
     p.wait_ns = 1000ull * unsigned(stall_us);
@@ -915,17 +1032,17 @@ int launch_umma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
   }
   const int tiles = p.tiles_m * p.tiles_n;
   const int grid = tiles < sm_count() ? tiles : sm_count();
-  kern<<<grid, kThreads, L::kDynamicBytes, st>>>(ta, tb, p);
+  kern<<<grid, kThreads, L::kDynamicBytes, st>>>(ta, tb, p, fx);
   return check_cuda(cudaGetLastError(), "a8w8 tcgen05 launch");
 }
 
 // Tile width BN with the stage count that fills shared memory for the rows of A a stage has to hold.
-template <typename OutT, int BN>
-int launch_umma_rows(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const A8W8Params& p, cudaStream_t st) {
+template <typename OutT, int BN, class FX = NoEpilogue>
+int launch_umma_rows(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const A8W8Params& p, cudaStream_t st, const FX& fx = FX{}) {
   constexpr int kBudget = 210 * 1024;
-  if (p.M <= 16) return launch_umma<OutT, BN, kBudget / ((16 + BN) * kBK), 16>(a, lda, b, ldb, p, st);
-  if (p.M <= 64) return launch_umma<OutT, BN, kBudget / ((64 + BN) * kBK), 64>(a, lda, b, ldb, p, st);
-  return launch_umma<OutT, BN, kBudget / ((kBM + BN) * kBK) < 8 ? kBudget / ((kBM + BN) * kBK) : 8, kBM>(a, lda, b, ldb, p, st);
+  if (p.M <= 16) return launch_umma<OutT, BN, kBudget / ((16 + BN) * kBK), 16>(a, lda, b, ldb, p, fx, st);
+  if (p.M <= 64) return launch_umma<OutT, BN, kBudget / ((64 + BN) * kBK), 64>(a, lda, b, ldb, p, fx, st);
+  return launch_umma<OutT, BN, kBudget / ((kBM + BN) * kBK) < 8 ? kBudget / ((kBM + BN) * kBK) : 8, kBM>(a, lda, b, ldb, p, fx, st);
 }
 
 // Geometry of the K-balanced mode for `tiles` 256-wide tiles of `kbs` K blocks on `pairs` CTA pairs.
@@ -969,17 +1086,18 @@ inline unsigned long long next_sk_epoch() {
   return e;
 }
 
-template <typename OutT, int BN, bool SK = false, int EPI = 4>
+template <typename OutT, int BN, bool SK = false, int EPI = 4, class FX = NoEpilogue>
 int launch_pair(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8Params p, cudaStream_t st,
-                void* workspace = nullptr) {
+                void* workspace = nullptr, const FX& fx = FX{}) {
+  constexpr int OW = FX::kGated ? BN / 2 : BN;
   // for the operand ring; the output staging buffers and the column scales of the epilogue warps take the rest
   constexpr int kBudget = (EPI == 4 ? 196 : 194) * 1024;
   constexpr int STAGES = kBudget / (kBM * kBK + (BN / 2) * kBK) < 8 ? kBudget / (kBM * kBK + (BN / 2) * kBK) : 8;
-  using L = PairSmem<BN, STAGES, EPI>;
+  using L = PairSmem<BN, STAGES, EPI, FX::kOn>;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
   static_assert(L::kStageBytes % 1024 == 0 && L::kABytes % 1024 == 0 && L::kOutOff % 1024 == 0, "tiles must stay 1024-byte aligned");
   static_assert(BN % 32 == 0 && BN <= 256, "pair tile width");
-  auto kern = a8w8_umma_pair_kernel<OutT, BN, STAGES, SK, false, EPI>;
+  auto kern = a8w8_umma_pair_kernel<OutT, BN, STAGES, SK, false, EPI, FX>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];  // per device, so that a failure is reported on every call and not only the first
   int dev = 0;
@@ -991,7 +1109,9 @@ int launch_pair(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(a8w8 pair)");
   CUtensorMap ta, tb, tout;
   if (int e = make_tmap_i8(&ta, a, p.M, p.K, lda, kBM)) return e;
-  if (int e = make_tmap_i8(&tb, b, p.N, p.K, ldb, BN / 2)) return e;
+  int64_t weight_rows = p.N;
+  if constexpr (FX::kOn) weight_rows = fx.rows;
+  if (int e = make_tmap_i8(&tb, b, weight_rows, p.K, ldb, BN / 2)) return e;
   // output blocks of 32 rows x 32 columns (64 bytes per row) for the epilogue's TMA stores, where the output allows it
   p.out_tma = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && ((p.ldo * int64_t(sizeof(OutT))) % 16 == 0);
   if (p.out_tma) {
@@ -1000,7 +1120,7 @@ int launch_pair(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
     tout = ta;  // never used
   }
   p.tiles_m = (p.M + 255) / 256;
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_n = (p.N + OW - 1) / OW;
   p.k_blocks = (p.K + kBK - 1) / kBK;
   const int tiles = p.tiles_m * p.tiles_n;
   int pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
@@ -1017,7 +1137,7 @@ int launch_pair(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
     p.sk_partials = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + kSkFlagBytes);
     p.sk_epoch = next_sk_epoch();
   }
-  kern<<<2 * pairs, (2 + EPI) * 32, L::kDynamicBytes, st>>>(ta, tb, tout, p);
+  kern<<<2 * pairs, (2 + EPI) * 32, L::kDynamicBytes, st>>>(ta, tb, tout, p, fx);
   return check_cuda(cudaGetLastError(), "a8w8 tcgen05 (CTA pair) launch");
 }
 
@@ -1046,7 +1166,7 @@ constexpr double kSkHandOverBlocks = 8.0;
 constexpr int kSkMinTailBlocks = 24;
 constexpr double kSkMinGain = 0.95;  // taken when at least 5 % cheaper than the best whole-tile plan
 
-inline A8W8Plan plan_a8w8(int M, int N, int sms);
+inline A8W8Plan plan_a8w8(int M, int N, int sms, bool gated = false);
 
 inline A8W8Plan plan_a8w8(int M, int N, int K, int sms, int balanced_mode /* 0 auto, 1 always where possible, 2 never */) {
   A8W8Plan best = plan_a8w8(M, N, sms);
@@ -1067,7 +1187,10 @@ inline A8W8Plan plan_a8w8(int M, int N, int K, int sms, int balanced_mode /* 0 a
   return best;
 }
 
-inline A8W8Plan plan_a8w8(int M, int N, int sms) {
+// gated: N output columns with a gate, so a tile of bn accumulator columns covers bn / 2 of them; half a tile has to be whole
+// chunks of 32 columns, which leaves out the widths 224 and 160
+inline A8W8Plan plan_a8w8(int M, int N, int sms, bool gated) {
+  if (gated) N *= 2;  // accumulator columns
   A8W8Plan best{false, 64, 1e30};
   const int tiles_m1 = (M + kBM - 1) / kBM;
   if (M <= kBM) {
@@ -1095,6 +1218,7 @@ inline A8W8Plan plan_a8w8(int M, int N, int sms) {
     const int tiles_m2 = (M + 255) / 256;
     for (int i = 0; i < 5; ++i) {
       const int bn = kPairWidths[i];
+      if (gated && bn % 64 != 0) continue;
       const long long tiles = 1ll * tiles_m2 * ((N + bn - 1) / bn);
       const double cost = double((tiles + pairs - 1) / pairs) * bn * kPairColumnCost[i];
       if (cost < best.cost) best = A8W8Plan{true, bn, cost};  // ties keep the wider tile (listed first)
@@ -1121,11 +1245,12 @@ __global__ void moe_gather_rows_kernel(const int8_t* __restrict__ a, int64_t lda
   for (int i = lane; i < K / 16; i += 32) dst[i] = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
 }
 
-template <typename OutT, int BN, int STAGES, int AROWS>
-int launch_moe(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A8W8Params p, cudaStream_t st) {
-  using L = SmemLayout<BN, STAGES, AROWS>;
+template <typename OutT, int BN, int STAGES, int AROWS, class FX>
+int launch_moe(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A8W8Params p, const FX& fx, cudaStream_t st) {
+  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn>;
+  constexpr int OW = FX::kGated ? BN / 2 : BN;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
-  auto kern = a8w8_umma_kernel<OutT, BN, STAGES, true, AROWS>;
+  auto kern = a8w8_umma_kernel<OutT, BN, STAGES, true, AROWS, FX>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];  // per device, so that a failure is reported on every call and not only the first
   int dev = 0;
@@ -1137,33 +1262,36 @@ int launch_moe(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(fused moe a8w8)");
   CUtensorMap ta, tb;
   if (int e = make_tmap_i8(&ta, a_sorted, EM, p.K, p.K, AROWS)) return e;  // a block's own slots (and a few more)
-  if (int e = make_tmap_i8(&tb, b, E * p.N, p.K, p.K, BN)) return e;
+  int64_t weight_rows = p.N;
+  if constexpr (FX::kOn) weight_rows = fx.rows;
+  if (int e = make_tmap_i8(&tb, b, E * weight_rows, p.K, p.K, OW)) return e;
   p.tiles_m = int(EM / p.tile_rows);
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_n = (p.N + OW - 1) / OW;
   p.k_blocks = (p.K + kBK - 1) / kBK;
   const int tiles = p.tiles_m * p.tiles_n;
   const int grid = tiles < sm_count() ? tiles : sm_count();
-  kern<<<grid, kThreads, L::kDynamicBytes, st>>>(ta, tb, p);
+  kern<<<grid, kThreads, L::kDynamicBytes, st>>>(ta, tb, p, fx);
   return check_cuda(cudaGetLastError(), "fused moe a8w8 launch");
 }
 
-template <typename OutT, int BN>
-int launch_moe_rows(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, const A8W8Params& p, cudaStream_t st) {
+template <typename OutT, int BN, class FX = NoEpilogue>
+int launch_moe_rows(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, const A8W8Params& p, cudaStream_t st, const FX& fx = FX{}) {
   constexpr int kBudget = 210 * 1024;
-  if (p.tile_rows <= 16) return launch_moe<OutT, BN, kBudget / ((16 + BN) * kBK), 16>(a_sorted, EM, b, E, p, st);
-  if (p.tile_rows <= 64) return launch_moe<OutT, BN, kBudget / ((64 + BN) * kBK), 64>(a_sorted, EM, b, E, p, st);
-  return launch_moe<OutT, BN, kBudget / ((kBM + BN) * kBK) < 8 ? kBudget / ((kBM + BN) * kBK) : 8, kBM>(a_sorted, EM, b, E, p, st);
+  if (p.tile_rows <= 16) return launch_moe<OutT, BN, kBudget / ((16 + BN) * kBK), 16>(a_sorted, EM, b, E, p, fx, st);
+  if (p.tile_rows <= 64) return launch_moe<OutT, BN, kBudget / ((64 + BN) * kBK), 64>(a_sorted, EM, b, E, p, fx, st);
+  return launch_moe<OutT, BN, kBudget / ((kBM + BN) * kBK) < 8 ? kBudget / ((kBM + BN) * kBK) : 8, kBM>(a_sorted, EM, b, E, p, fx, st);
 }
 
 // Blocks of 256 sorted slots (or a multiple): one block is one 256-row tile of the CTA-pair kernel.
-template <typename OutT>
-int launch_moe_pair(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A8W8Params p, cudaStream_t st) {
+template <typename OutT, int EPI = 4, class FX = NoEpilogue>
+int launch_moe_pair(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A8W8Params p, cudaStream_t st, const FX& fx = FX{}) {
   constexpr int BN = 256;
-  constexpr int kBudget = 196 * 1024;
+  constexpr int OW = FX::kGated ? BN / 2 : BN;
+  constexpr int kBudget = (EPI == 4 ? 196 : 194) * 1024;
   constexpr int STAGES = kBudget / (kBM * kBK + (BN / 2) * kBK);
-  using L = PairSmem<BN, STAGES>;
+  using L = PairSmem<BN, STAGES, EPI, FX::kOn>;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
-  auto kern = a8w8_umma_pair_kernel<OutT, BN, STAGES, false, true>;
+  auto kern = a8w8_umma_pair_kernel<OutT, BN, STAGES, false, true, EPI, FX>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];  // per device, so that a failure is reported on every call and not only the first
   int dev = 0;
@@ -1175,14 +1303,16 @@ int launch_moe_pair(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(fused moe a8w8, CTA pair)");
   CUtensorMap ta, tb;
   if (int e = make_tmap_i8(&ta, a_sorted, EM, p.K, p.K, kBM)) return e;
-  if (int e = make_tmap_i8(&tb, b, E * p.N, p.K, p.K, BN / 2)) return e;
+  int64_t weight_rows = p.N;
+  if constexpr (FX::kOn) weight_rows = fx.rows;
+  if (int e = make_tmap_i8(&tb, b, E * weight_rows, p.K, p.K, BN / 2)) return e;
   p.tiles_m = int(EM / 256);
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_n = (p.N + OW - 1) / OW;
   p.k_blocks = (p.K + kBK - 1) / kBK;
   p.out_tma = 0;
   const int tiles = p.tiles_m * p.tiles_n;
   const int pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  kern<<<2 * pairs, kThreads, L::kDynamicBytes, st>>>(ta, tb, ta, p);
+  kern<<<2 * pairs, (2 + EPI) * 32, L::kDynamicBytes, st>>>(ta, tb, ta, p, fx);
   return check_cuda(cudaGetLastError(), "fused moe a8w8 (CTA pair) launch");
 }
 

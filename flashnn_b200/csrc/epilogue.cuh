@@ -1,0 +1,106 @@
+// What an A8W8 product does with its scaled sums before their one rounding to the output type: bias, activation, gate
+// and residual, all in fp32.
+//
+//   plain   out = T(act(v[n]) + r[m, n])                with v = fl32(acc * s) + bias
+//   gated   out = T(act(v[n]) * v[N + n] + r[m, n])     the weight has 2 N rows: the N rows inside the activation, then
+//                                                       the N rows that its value multiplies
+//
+// The gate needs the sums of weight rows n and N + n in one thread, so a gated tile of BN accumulator columns takes
+// BN / 2 rows from each half of the weight: the two halves meet in the accumulator, and the output, half as wide as the
+// product, is all that leaves the chip.
+#pragma once
+#include "common.cuh"
+#include "quantise.cuh"
+
+namespace fnn {
+
+// kernels without an epilogue of this kind
+struct NoEpilogue {
+  static constexpr bool kOn = false, kGated = false;
+};
+template <bool GATED> struct FusedEpilogue {
+  static constexpr bool kOn = true, kGated = GATED;
+  const void* bias;      // nullptr or [rows] (fused MoE: [E, rows])
+  const void* residual;  // nullptr or [M, N] in the output's dtype
+  int64_t ldr;
+  int bias_dtype, act;   // act: fnn_activation
+  int rows;              // weight rows (of one expert): N, or 2 N with a gate
+  int experts;           // fused MoE: slots of a block whose expert is not one of these write nothing
+};
+
+// 1 / (1 + e^-v) by the hardware's exponential and reciprocal: a few 2^-22 off, far below the half step (2^-9, 2^-12) of
+// the 16-bit output.  e^-v of a very negative v is infinite and its reciprocal 0; a NaN stays one.
+__device__ __forceinline__ float sigmoid_f32(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
+template <int ACT> __device__ __forceinline__ float activate(float v) {
+  if (ACT == FNN_ACT_RELU) return v < 0.f ? 0.f : v;  // (keeps a NaN)
+  if (ACT == FNN_ACT_SIGMOID) return sigmoid_f32(v);
+  if (ACT == FNN_ACT_SILU) return v * sigmoid_f32(v);
+  if (ACT == FNN_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  // v / 2 (1 + tanh(t)) = v sigmoid(2 t)
+  if (ACT == FNN_ACT_GELU_TANH) return v * sigmoid_f32(1.5957691216057308f * fmaf(0.044715f * v, v * v, v));
+  return v;
+}
+template <int ACT, int N> __device__ __forceinline__ void activate_all(float (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = activate<ACT>(v[j]);
+}
+// the activation is a launch argument: one uniform branch for a thread's N values
+template <int N> __device__ __forceinline__ void activate_n(float (&v)[N], int act) {
+  switch (act) {
+    case FNN_ACT_RELU: activate_all<FNN_ACT_RELU>(v); break;
+    case FNN_ACT_SIGMOID: activate_all<FNN_ACT_SIGMOID>(v); break;
+    case FNN_ACT_SILU: activate_all<FNN_ACT_SILU>(v); break;
+    case FNN_ACT_GELU: activate_all<FNN_ACT_GELU>(v); break;
+    case FNN_ACT_GELU_TANH: activate_all<FNN_ACT_GELU_TANH>(v); break;
+    default: break;
+  }
+}
+__device__ __forceinline__ float activate_one(float v, int act) {
+  float a[1] = {v};
+  activate_n(a, act);
+  return a[0];
+}
+
+// 32 consecutive residual values of one row as packed pairs; zeros outside the matrix
+template <typename T, class FX>
+__device__ __forceinline__ void load_residual32(const FX& fx, int row, int col0, int M, int N, bool vec_ok, uint32_t (&r)[16]) {
+  if constexpr (FX::kOn) {
+    if (row >= M || col0 >= N) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = 0u;
+      return;
+    }
+    const T* src = reinterpret_cast<const T*>(fx.residual) + int64_t(row) * fx.ldr + col0;
+    if (vec_ok && col0 + 32 <= N) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 u = *reinterpret_cast<const uint4*>(src + 8 * j);
+        r[4 * j] = u.x; r[4 * j + 1] = u.y; r[4 * j + 2] = u.z; r[4 * j + 3] = u.w;
+      }
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t lo = col0 + 2 * j < N ? h[2 * j] : 0u, hi = col0 + 2 * j + 1 < N ? h[2 * j + 1] : 0u;
+        r[j] = lo | (hi << 16);
+      }
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ void add_residual32(const uint32_t (&r)[16], float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    v[2 * j] += lo_of<T>(r[j]);
+    v[2 * j + 1] += hi_of<T>(r[j]);
+  }
+}
+__device__ __forceinline__ void add_bias32(const float* b, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 t = *reinterpret_cast<const float4*>(b + j);
+    v[j] += t.x; v[j + 1] += t.y; v[j + 2] += t.z; v[j + 3] += t.w;
+  }
+}
+
+}  // namespace fnn

@@ -29,6 +29,7 @@
 // into the MMA operand as they are) and an 8-step FIFO of the same size in bytes.
 #include "async_copy.cuh"
 #include "common.cuh"
+#include "epilogue.cuh"
 #include "weight_only.cuh"
 
 namespace fnn {
@@ -122,9 +123,13 @@ __device__ __forceinline__ void imma0(int (&d)[4], uint32_t a0, uint32_t a1, uin
 // group) stay in registers instead of being re-read from shared memory at every step.
 // A8: the activations are int8 already (A8W8 decode): they are copied into the planes as they are, one column per
 // token, the int32 sums stay exact all the way to the reducer, which applies the A8W8 scaling rule.
-template <typename T, int BITS, int NF, int SPU, bool PERCH, bool GZP, int DEPTH, bool XREG, bool A8 = false>
+// FX (A8 only): the fused epilogue of epilogue.cuh, applied by the reducer.  With a gate a row group is 8 output columns:
+// MMA rows 0-7 are the weight rows inside the activation, rows 8-15 those that its value multiplies, so the two sums of an
+// output meet in the reducer and the weight stream is as dense as without one.
+template <typename T, int BITS, int NF, int SPU, bool PERCH, bool GZP, int DEPTH, bool XREG, bool A8 = false, class FX = NoEpilogue>
 __global__ void __launch_bounds__(kImmaCtaThreads, 1)
-gemv_w4_imma_kernel(const WoParams p, const int num_rg) {
+gemv_w4_imma_kernel(const WoParams p, const int num_rg, const FX fx) {
+  static_assert(A8 || !FX::kOn, "the fused epilogue is for int8 activations");
   constexpr int kImmaSlotBytes = imma_slot_bytes(BITS);
   constexpr bool W8 = BITS == 8;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -152,12 +157,14 @@ gemv_w4_imma_kernel(const WoParams p, const int num_rg) {
   const uint32_t fifo = smem_u32(smem) + warp * (DEPTH * kImmaSlotBytes) + lane * 16;
   // weight rows of a row group: 8 packed rows (int4) or 16 rows (int8); this lane reads packed row g, or rows 2g and
   // 2g + 1, which are MMA rows g and g + 8 in both cases (channels 2g and 2g + 1 of the group)
-  const int64_t rg_stride = int64_t(gridDim.x) * (W8 ? 16 : 8) * K;
+  constexpr int kGroupRows = (W8 && !FX::kGated) ? 16 : 8;      // consecutive weight rows of a row group
+  const int64_t rg_stride = int64_t(gridDim.x) * kGroupRows * K;
   // fill cursor: the next block of this CTA's work to request; it runs kRingBlocks blocks ahead of the consumer
-  const uint8_t* wfill = p.qw + (int64_t(blockIdx.x) * (W8 ? 16 : 8) + (W8 ? 2 * g : g)) * K + k_begin + tig * 16;
+  const uint8_t* wfill = p.qw + (int64_t(blockIdx.x) * kGroupRows + (W8 && !FX::kGated ? 2 * g : g)) * K + k_begin + tig * 16;
+  const int64_t second_row = (FX::kGated ? int64_t(p.N) : 1) * K;  // (a gated group's second row is N rows on)
   auto copy_step = [&](uint32_t slot_addr, const uint8_t* w) {
     cp_async16(slot_addr, w);
-    if (W8) cp_async16(slot_addr + 512, w + K);
+    if (W8) cp_async16(slot_addr + 512, w + (FX::kGated ? second_row : K));
   };
   int fill_rg = worker ? int(blockIdx.x) : num_rg, fill_blk = 0;  // (the reducer warp never requests anything)
   const int64_t fill_wrap = rg_stride - int64_t(nblk - 1) * (kImmaBlk * kImmaStepK);  // last block -> first of the next row group
@@ -338,11 +345,28 @@ gemv_w4_imma_kernel(const WoParams p, const int num_rg) {
         __syncwarp();
         T* out = reinterpret_cast<T*>(p.out);
         const bool same16 = (p.row_dtype == p.scale_dtype) && (p.row_dtype != FNN_F32);
-        for (int idx = lane; idx < 16 * M; idx += 32) {
-          const int cl = idx & 15, tok = idx >> 4;
-          const int row = (cl & 1) ? (cl >> 1) + 8 : (cl >> 1);
+        auto scaled = [&](int row, int tok, int ch) {  // (fused epilogue: with the bias)
+          float sc = __fmul_rn(load_as_f32(p.row_scale, p.row_dtype, tok), load_as_f32(p.scale, p.scale_dtype, ch));
+          if (same16) sc = round_through(sc, p.row_dtype);
+          float v = __fmul_rn(float(fi[row * 16 + tok]), sc);
+          if constexpr (FX::kOn) {
+            if (fx.bias) v += load_as_f32(fx.bias, fx.bias_dtype, ch);
+          }
+          return v;
+        };
+        constexpr int kGroupCols = FX::kGated ? 8 : 16;
+        for (int idx = lane; idx < kGroupCols * M; idx += 32) {
+          const int cl = idx % kGroupCols, tok = idx / kGroupCols;
+          const int row = FX::kGated ? cl : (cl & 1) ? (cl >> 1) + 8 : (cl >> 1);
+          const int ch = rg * kGroupCols + cl;
+          if constexpr (FX::kOn) {
+            float v = activate_one(scaled(row, tok, ch), fx.act);
+            if (FX::kGated) v *= scaled(row + 8, tok, p.N + ch);
+            if (fx.residual) v += to_f32(reinterpret_cast<const T*>(fx.residual)[int64_t(tok) * fx.ldr + ch]);
+            out[int64_t(tok) * p.ldo + ch] = from_f32<T>(v);
+            continue;
+          }
           const int acc = fi[row * 16 + tok];
-          const int ch = rg * 16 + cl;
           if (p.acc_out) p.acc_out[int64_t(tok) * p.ldacc + ch] = acc;
           float sc = __fmul_rn(load_as_f32(p.row_scale, p.row_dtype, tok), load_as_f32(p.scale, p.scale_dtype, ch));
           if (same16) sc = round_through(sc, p.row_dtype);
@@ -543,7 +567,7 @@ int launch_imma_x(const WoParams& p, size_t smem_bytes, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = opt_static_weights() ? 1 : 0;
-  return check_cuda(cudaLaunchKernelEx(&cfg, gemv_w4_imma_kernel<T, BITS, NF, SPU, PERCH, GZP, DEPTH, XREG>, p, num_rg),
+  return check_cuda(cudaLaunchKernelEx(&cfg, gemv_w4_imma_kernel<T, BITS, NF, SPU, PERCH, GZP, DEPTH, XREG>, p, num_rg, NoEpilogue{}),
                     "weight-only decode (integer tensor pipe) launch");
 }
 
@@ -574,9 +598,9 @@ int launch_imma_shape(const WoParams& p, int spu, int nf, int depth, size_t smem
   return depth == kDeep ? launch_imma_spu<T, BITS, 2, kDeep>(p, spu, smem_bytes, st) : launch_imma_spu<T, BITS, 2, kShallow>(p, spu, smem_bytes, st);
 }
 
-template <typename T, int NF, int DEPTH, bool XREG>
-int launch_a8(const WoParams& p, size_t smem_bytes, cudaStream_t st) {
-  auto kern = gemv_w4_imma_kernel<T, 8, NF, 4, true, false, DEPTH, XREG, true>;
+template <typename T, int NF, int DEPTH, bool XREG, class FX>
+int launch_a8(const WoParams& p, size_t smem_bytes, const FX& fx, cudaStream_t st) {
+  auto kern = gemv_w4_imma_kernel<T, 8, NF, 4, true, false, DEPTH, XREG, true, FX>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -585,29 +609,30 @@ int launch_a8(const WoParams& p, size_t smem_bytes, cudaStream_t st) {
     if (err != cudaSuccess) return check_cuda(err, "a8w8 decode kernel attribute");
     configured[dev & 63] = true;
   }
-  const int num_rg = p.N / 16;
+  const int num_rg = p.N / (FX::kGated ? 8 : 16);
   const int cap = sm_count();
   const int rounds = (num_rg + cap - 1) / cap;
   const int grid = (num_rg + rounds - 1) / rounds;
-  kern<<<grid, kImmaCtaThreads, smem_bytes, st>>>(p, num_rg);
+  kern<<<grid, kImmaCtaThreads, smem_bytes, st>>>(p, num_rg, fx);
   return check_cuda(cudaGetLastError(), "a8w8 decode (integer tensor pipe) launch");
 }
 
-template <typename T>
-int launch_a8_shape(const WoParams& p, int nf, int depth, size_t smem_bytes, cudaStream_t st) {
+template <typename T, class FX>
+int launch_a8_shape(const WoParams& p, int nf, int depth, size_t smem_bytes, const FX& fx, cudaStream_t st) {
   if (nf == 1) {
-    if (depth == 8) return p.K == 8192 ? launch_a8<T, 1, 8, true>(p, smem_bytes, st) : launch_a8<T, 1, 8, false>(p, smem_bytes, st);
-    return launch_a8<T, 1, 4, false>(p, smem_bytes, st);
+    if (depth == 8) return p.K == 8192 ? launch_a8<T, 1, 8, true>(p, smem_bytes, fx, st) : launch_a8<T, 1, 8, false>(p, smem_bytes, fx, st);
+    return launch_a8<T, 1, 4, false>(p, smem_bytes, fx, st);
   }
-  return depth == 8 ? launch_a8<T, 2, 8, false>(p, smem_bytes, st) : launch_a8<T, 2, 4, false>(p, smem_bytes, st);
+  if constexpr (!FX::kOn)  // (a fused epilogue comes with at most 8 tokens)
+    return depth == 8 ? launch_a8<T, 2, 8, false>(p, smem_bytes, fx, st) : launch_a8<T, 2, 4, false>(p, smem_bytes, fx, st);
+  return -1;
 }
 
-}  // namespace
-
-int gemv_a8w8_imma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const void* alpha_row, int row_dtype,
-                   const void* alpha_col, int col_dtype, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
-                   int32_t* acc_out, int64_t ldacc, cudaStream_t st) {
-  if (M < 1 || M > 16 || N % 16 != 0 || K % (kImmaStepK * kImmaWarps * kImmaBlk) != 0 || ldb != K) return -1;
+template <class FX>
+int gemv_a8w8(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const void* alpha_row, int row_dtype,
+              const void* alpha_col, int col_dtype, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+              int32_t* acc_out, int64_t ldacc, const FX& fx, cudaStream_t st) {
+  if (M < 1 || M > 16 || N % (FX::kGated ? 8 : 16) != 0 || K % (kImmaStepK * kImmaWarps * kImmaBlk) != 0 || ldb != K) return -1;
   if (reinterpret_cast<uintptr_t>(a) % 16 != 0 || lda % 16 != 0 || reinterpret_cast<uintptr_t>(b) % 16 != 0) return -1;
   if (K / kImmaWarps > 65536) return -1;  // |acc| of a warp's K slice stays below 2^31
   WoParams p{};
@@ -623,9 +648,32 @@ int gemv_a8w8_imma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, c
     L = imma_layout(8, M, K, nf, depth, 0, 0, 1);
   }
   if (L.total > kImmaSmemCap) return -1;
-  if (out_dtype == FNN_F16) return launch_a8_shape<__half>(p, nf, depth, L.total, st);
-  return launch_a8_shape<__nv_bfloat16>(p, nf, depth, L.total, st);
+  if (out_dtype == FNN_F16) return launch_a8_shape<__half>(p, nf, depth, L.total, fx, st);
+  return launch_a8_shape<__nv_bfloat16>(p, nf, depth, L.total, fx, st);
 }
+
+}  // namespace
+
+int gemv_a8w8_imma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const void* alpha_row, int row_dtype,
+                   const void* alpha_col, int col_dtype, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                   int32_t* acc_out, int64_t ldacc, cudaStream_t st) {
+  return gemv_a8w8(a, lda, b, ldb, alpha_row, row_dtype, alpha_col, col_dtype, out, out_dtype, ldo, M, N, K, acc_out, ldacc,
+                   NoEpilogue{}, st);
+}
+
+template <class FX>
+int gemv_a8w8_imma_fused(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const void* alpha_row, int row_dtype,
+                         const void* alpha_col, int col_dtype, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                         const FX& fx, cudaStream_t st) {
+  if (M > 8) return -1;
+  return gemv_a8w8(a, lda, b, ldb, alpha_row, row_dtype, alpha_col, col_dtype, out, out_dtype, ldo, M, N, K, nullptr, 0, fx, st);
+}
+template int gemv_a8w8_imma_fused<FusedEpilogue<false>>(const int8_t*, int64_t, const int8_t*, int64_t, const void*, int, const void*,
+                                                        int, void*, int, int64_t, int, int, int, const FusedEpilogue<false>&,
+                                                        cudaStream_t);
+template int gemv_a8w8_imma_fused<FusedEpilogue<true>>(const int8_t*, int64_t, const int8_t*, int64_t, const void*, int, const void*,
+                                                       int, void*, int, int64_t, int, int, int, const FusedEpilogue<true>&,
+                                                       cudaStream_t);
 
 int gemv_w4_imma(const WoParams& p, int bits, int act_dtype, cudaStream_t st) {
   if (p.M < 1 || p.M > kImmaMaxTokens) return -1;

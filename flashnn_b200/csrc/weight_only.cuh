@@ -41,6 +41,12 @@ int gemv_a8w8_imma(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, c
                    const void* alpha_col, int col_dtype, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
                    int32_t* acc_out, int64_t ldacc, cudaStream_t st);
 
+// The same for at most 8 tokens with a fused epilogue (epilogue.cuh); with a gate b is [2 N, K].
+template <class FX>
+int gemv_a8w8_imma_fused(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const void* alpha_row, int row_dtype,
+                         const void* alpha_col, int col_dtype, void* out, int out_dtype, int64_t ldo, int M, int N, int K,
+                         const FX& fx, cudaStream_t st);
+
 // Fused MoE with packed-int4 expert weights on the prefill (tcgen05) kernels of gemm_weight_only.cu, for blocks of 256
 // sorted slots or a multiple.  Returns an fnn_status, or -1 when the shape, the alignment or the workspace is outside
 // what they take.  The workspace holds the expert-sorted copy of the token rows (and their row sums with zero-points).

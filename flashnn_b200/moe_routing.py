@@ -1,0 +1,111 @@
+"""The two ends of a mixture-of-experts layer: MoeRouting turns router logits into each token's experts and weights,
+moe_sort_tokens turns those into the block-aligned slot list that the expert products (fused_moe_a8w8_forward,
+fused_moe_a8w8_gated_forward, fused_moe_a16w4_forward) read, and moe_combine sums their [M, top_k, N] output over a
+token's choices."""
+import torch
+
+from . import _lib
+from .fused_moe import _i32
+from .kernel_backend import BackendKernel
+from .quant_gemm import _DT, _on_device, _require_cuda, _stream
+
+
+class MoeRouting(BackendKernel):
+    """forward(logits [M, E] fp16/bf16/fp32, bias=None or [E]) -> (topk_weights [M, top_k] fp32, topk_ids [M, top_k] int32)
+
+    score = softmax(logits) or sigmoid(logits); the experts with the `top_k` largest score + bias are chosen, best first,
+    equal ones by the lowest index; their weights are the scores (without the bias), divided by their sum if `renormalize`,
+    times `scale`.  With num_groups > 1 only the experts of the best `topk_groups` groups of E / num_groups consecutive ones
+    can be chosen; a group's score is the largest score + bias in it ("max") or the sum of its two largest ("top2").
+    The order is that of 64-bit arithmetic.  A logit of -inf takes an expert out (under the sigmoid with a bias: a bias of
+    -inf), while top_k others are left."""
+
+    def __init__(self, num_experts: int, top_k: int, scoring: str = "softmax", renormalize: bool = True, num_groups: int = 1,
+                 topk_groups: int = 1, group_score: str = "max", scale: float = 1.0):
+        super().__init__()
+        assert scoring in _lib.SCORINGS, f"unknown scoring {scoring!r}"
+        assert group_score in _lib.GROUP_SCORES, f"unknown group score {group_score!r}"
+        assert num_groups >= 1 and num_experts % num_groups == 0, "num_groups must divide num_experts"
+        assert 1 <= topk_groups <= num_groups, "topk_groups must be between 1 and num_groups"
+        assert 1 <= top_k <= topk_groups * (num_experts // num_groups), "top_k must not exceed the experts of the chosen groups"
+        self.num_experts, self.top_k = num_experts, top_k
+        self.scoring, self.renormalize, self.scale = scoring, bool(renormalize), float(scale)
+        self.num_groups, self.topk_groups, self.group_score = num_groups, topk_groups, group_score
+
+    def _cuda_impl(self, logits, bias=None):
+        _require_cuda(logits, bias)
+        assert logits.dim() == 2 and logits.shape[1] == self.num_experts, "logits must be [M, num_experts]"
+        assert logits.dtype in _DT, "logits must be float16, bfloat16 or float32"
+        m, e = logits.shape
+        if e > 1 and logits.stride(1) != 1:
+            logits = logits.contiguous()
+        if bias is not None:
+            assert bias.numel() == e and bias.is_floating_point(), "bias must be [num_experts]"
+            bias = bias.reshape(-1).to(torch.float32).contiguous()
+        weights = torch.empty((m, self.top_k), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((m, self.top_k), dtype=torch.int32, device=logits.device)
+        with _on_device(logits):
+            _lib.check(_lib.lib().fnn_moe_route(
+                logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if m > 1 else e, m, e,
+                bias.data_ptr() if bias is not None else None, _lib.SCORINGS[self.scoring], int(self.renormalize),
+                self.num_groups, self.topk_groups, _lib.GROUP_SCORES[self.group_score], self.scale, self.top_k,
+                weights.data_ptr(), ids.data_ptr(), _stream(logits)))
+        return weights, ids
+
+    def forward(self, logits, bias=None):
+        return BackendKernel.forward(self, logits, bias)
+
+
+def moe_sort_tokens(topk_ids, num_experts, BM, first_expert=0):
+    """topk_ids [M, top_k] -> (sorted_token_ids [EM], expert_ids [EM / BM], num_tokens_post_padded [1]), int32: the flat
+    (token, choice) indices grouped by expert in ascending order, every group padded to a multiple of BM with M * top_k.
+
+    Experts are first_expert .. first_expert + num_experts - 1 and numbered from 0 in expert_ids; a choice of any other
+    expert (one of another device, or -1) gets no slot.  EM depends on the sizes alone: the most slots that any choice of
+    experts fills."""
+    _require_cuda(topk_ids)
+    assert topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64"
+    assert num_experts >= 1 and BM >= 1, "num_experts and BM must be positive"
+    ids = _i32(topk_ids).contiguous()
+    L = _lib.lib()
+    em = L.fnn_moe_sort_slots(ids.numel(), num_experts, BM)
+    sorted_ids = torch.empty(em, dtype=torch.int32, device=ids.device)
+    experts = torch.empty(em // BM, dtype=torch.int32, device=ids.device)
+    in_use = torch.empty(1, dtype=torch.int32, device=ids.device)
+    with _on_device(ids):
+        _lib.check(L.fnn_moe_sort(ids.data_ptr(), ids.numel(), num_experts, first_expert, BM, sorted_ids.data_ptr(), em,
+                                  experts.data_ptr(), in_use.data_ptr(), _stream(ids)))
+    return sorted_ids, experts, in_use
+
+
+def moe_combine(C, topk_weights=None, topk_ids=None, num_experts=None, first_expert=0, residual=None):
+    """C [M, top_k, N] fp16/bf16 -> [M, N] in C's dtype: the sum over a token's choices, times topk_weights [M, top_k] where
+    given (the expert products can have applied them), plus residual [M, N], in fp32 and rounded once.
+
+    With topk_ids [M, top_k] choices of experts outside first_expert .. first_expert + num_experts - 1 are left out: the
+    expert products did not write their rows of C, which are not read."""
+    _require_cuda(C, topk_weights, topk_ids, residual)
+    assert C.dim() == 3 and C.dtype in (torch.float16, torch.bfloat16), "C must be [M, top_k, N] in float16 or bfloat16"
+    m, k, n = C.shape
+    if n > 1 and C.stride(2) != 1:
+        C = C.contiguous()
+    if topk_weights is not None:
+        assert topk_weights.shape == (m, k) and topk_weights.dtype in _DT, "topk_weights must be [M, top_k] in a float dtype"
+        topk_weights = topk_weights.float().contiguous()
+    if topk_ids is not None:
+        assert topk_ids.shape == (m, k) and num_experts is not None and num_experts >= 1, "topk_ids must be [M, top_k], with num_experts"
+        topk_ids = _i32(topk_ids).contiguous()
+    ldr = 0
+    if residual is not None:
+        assert residual.shape == (m, n) and residual.dtype == C.dtype, "residual must be [M, N] in C's dtype"
+        if n > 1 and residual.stride(1) != 1:
+            residual = residual.contiguous()
+        ldr = residual.stride(0) if m > 1 else n
+    out = torch.empty((m, n), dtype=C.dtype, device=C.device)
+    with _on_device(C):
+        _lib.check(_lib.lib().fnn_moe_combine(
+            C.data_ptr(), _DT[C.dtype], C.stride(0) if m > 1 else k * n, C.stride(1) if k > 1 else n, m, k, n,
+            topk_weights.data_ptr() if topk_weights is not None else None, topk_ids.data_ptr() if topk_ids is not None else None,
+            num_experts if topk_ids is not None else 1, first_expert, residual.data_ptr() if residual is not None else None, ldr,
+            out.data_ptr(), n, _stream(C)))
+    return out

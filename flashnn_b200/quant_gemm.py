@@ -137,6 +137,63 @@ class GemmA8W8(BackendKernel):
         return BackendKernel.forward(self, a, b, alpha_row, alpha_col)
 
 
+class GemmA8W8Epilogue(BackendKernel):
+    """GemmA8W8 with bias, activation, gate and residual in its epilogue: with v = GemmA8W8's scaled sums + bias, in fp32,
+    out = act(v) + residual, or gated: out[:, n] = act(v[:, n]) * v[:, N + n] + residual, rounded once to `out_ty`.
+
+    forward(a int8 [M, K], b int8 [N, K], alpha_row [M] or [M, 1], alpha_col [N] or [1, N],
+            bias=None or [N], residual=None or [M, N] in out_ty) -> [M, N]
+    With gated=True b, alpha_col and bias have 2 N rows: the N rows inside the activation, then the N rows that its value
+    multiplies.  activation: None, "relu", "sigmoid", "silu", "gelu" (erf) or "gelu_tanh"."""
+
+    def __init__(self, out_ty: torch.dtype = torch.float16, activation=None, gated: bool = False):
+        super().__init__()
+        assert activation in _lib.ACTIVATIONS, f"unknown activation {activation!r}"
+        self.out_ty = out_ty
+        self.activation = activation
+        self.gated = bool(gated)
+
+    def _cuda_impl(self, a, b, alpha_row, alpha_col, bias=None, residual=None):
+        _require_cuda(a, b, alpha_row, alpha_col, bias, residual)
+        assert a.dim() == 2 and b.dim() == 2, "Matrix A/B must be 2-D"
+        assert a.dtype == torch.int8 and b.dtype == torch.int8, "Matrix A/B must be int8 type"
+        assert self.out_ty in (torch.float16, torch.bfloat16), "Output type must be float16 or bfloat16"
+        assert a.shape[1] == b.shape[1], "Matrix B must be transposed"
+        (m, k), rows = a.shape, b.shape[0]
+        assert not self.gated or rows % 2 == 0, "with a gate matrix B must have an even number of rows"
+        n = rows // 2 if self.gated else rows
+        if k > 1 and a.stride(1) != 1:
+            a = a.contiguous()
+        if k > 1 and b.stride(1) != 1:
+            b = b.contiguous()
+        row = alpha_row.reshape(-1).contiguous()
+        col = alpha_col.reshape(-1).contiguous()
+        assert row.numel() == m and col.numel() == rows, "scale shapes must be [M] and [N] (2 N with a gate)"
+        assert row.dtype in _DT and col.dtype in _DT, "scales must be float16, bfloat16 or float32"
+        if bias is not None:
+            bias = bias.reshape(-1).contiguous()
+            assert bias.numel() == rows and bias.dtype in _DT, "bias must be [N] (2 N with a gate) in a float dtype"
+        ldr = 0
+        if residual is not None:
+            assert residual.shape == (m, n) and residual.dtype == self.out_ty, "residual must be [M, N] in the output type"
+            if n > 1 and residual.stride(1) != 1:
+                residual = residual.contiguous()
+            ldr = residual.stride(0) if m > 1 else n
+        out = torch.empty([m, n], dtype=self.out_ty, device=a.device)
+        with _on_device(a):
+            _lib.check(_lib.lib().fnn_gemm_a8w8_epilogue(
+                a.data_ptr(), a.stride(0) if m > 1 else k, b.data_ptr(), b.stride(0) if rows > 1 else k,
+                row.data_ptr(), _DT[row.dtype], col.data_ptr(), _DT[col.dtype],
+                bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0,
+                _lib.ACTIVATIONS[self.activation], int(self.gated),
+                residual.data_ptr() if residual is not None else None, ldr,
+                out.data_ptr(), _DT[self.out_ty], n, m, n, k, _stream(a)))
+        return out
+
+    def forward(self, a, b, alpha_row, alpha_col, bias=None, residual=None):
+        return BackendKernel.forward(self, a, b, alpha_row, alpha_col, bias, residual)
+
+
 class GemmWeightOnly(BackendKernel):
     """out = act . dequant(quant_w)^T (+ bias) with int8 or packed-int4 weights.
 

@@ -48,6 +48,21 @@ typedef enum fnn_dtype {
   FNN_F32 = 2
 } fnn_dtype;
 
+/* Activations of the fused epilogues, computed in fp32.  silu(v) = v * sigmoid(v); gelu(v) = v / 2 * (1 + erf(v / sqrt 2));
+ * gelu_tanh(v) = v / 2 * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))).  A NaN stays a NaN. */
+typedef enum fnn_activation {
+  FNN_ACT_NONE = 0,
+  FNN_ACT_RELU = 1,
+  FNN_ACT_SIGMOID = 2,
+  FNN_ACT_SILU = 3,
+  FNN_ACT_GELU = 4,
+  FNN_ACT_GELU_TANH = 5
+} fnn_activation;
+
+/* How fnn_moe_route turns a logit into a score, and a group's keys into the group's. */
+typedef enum fnn_moe_scoring { FNN_SCORE_SOFTMAX = 0, FNN_SCORE_SIGMOID = 1 } fnn_moe_scoring;
+typedef enum fnn_moe_group_score { FNN_GROUP_MAX = 0, FNN_GROUP_TOP2 = 1 } fnn_moe_group_score;
+
 /*
  * Process-wide options (fnn_set_option / fnn_get_option).  No counterpart in the reference.
  *
@@ -174,6 +189,30 @@ size_t fnn_gemm_a8w8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int fnn_gemm_a8w8_plan(int64_t M, int64_t N, int64_t K, int* kernel, int* tile_n);
 
 /*
+ * A8W8 GEMM with bias, activation, gate and residual in its epilogue.  No counterpart in the reference, where each of them is
+ * a pass of its own over the output.  With v[m,r] = fl32(float(acc) * s) + bias[r], s as for fnn_gemm_a8w8:
+ *     gated == 0:  out[m,n] = act(v[m,n]) + residual[m,n]                b is [N, K]
+ *     gated != 0:  out[m,n] = act(v[m,n]) * v[m,N+n] + residual[m,n]     b is [2 N, K]: the N rows inside the activation,
+ *                                                                        then the N rows that its value multiplies
+ * all in fp32 and rounded once to out_dtype.  The accumulator is exact int32.
+ *
+ *   a          [M, K]  int8, lda      b          [N or 2 N, K]  int8, ldb
+ *   alpha_row  [M]     row_dtype      alpha_col  [N or 2 N]     col_dtype  (f16/bf16/f32)
+ *   bias       NULL or [N or 2 N] of bias_dtype (f16/bf16/f32)
+ *   activation an fnn_activation
+ *   residual   NULL or [M, N] in out_dtype, ldr (0: the same row for every m).  It may be `out` itself (same pointer,
+ *              ldr == ldo); otherwise the two do not overlap
+ *   out        [M, N]  f16 or bf16 (out_dtype), ldo
+ *
+ * Fast path: a, b 16-byte aligned and lda, ldb multiples of 16; anything else runs a slower generic kernel with the same
+ * results.  Needs no workspace.
+ */
+int fnn_gemm_a8w8_epilogue(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const void* alpha_row, int row_dtype,
+                           const void* alpha_col, int col_dtype, const void* bias, int bias_dtype, int activation, int gated,
+                           const void* residual, int64_t ldr, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N,
+                           int64_t K, void* stream);
+
+/*
  * Fused mixture-of-experts A8W8 GEMM over expert-sorted token slots.
  * Replaces `fused_moe_a8w8_forward(A, B, C, alpha_row, alpha_col, topk_weights, topk_ids, sorted_token_ids, expert_ids,
  * num_tokens_post_padded, mul_routed_weight, top_k, BM)` (flashnn/triton_kernels/fused_moe_a8w8.py:176-290; arithmetic
@@ -202,6 +241,77 @@ int fnn_fused_moe_a8w8(const int8_t* a, int64_t lda, const int8_t* b, int64_t E,
                        int top_k, int block_m, int mul_routed_weight, void* out, int out_dtype, int64_t ldo,
                        void* workspace, size_t workspace_bytes, void* stream);
 size_t fnn_fused_moe_a8w8_workspace_bytes(int64_t EM, int64_t K);
+
+/*
+ * The first half of the experts' feed-forward networks: the product of fnn_fused_moe_a8w8 with the activation and the gate in
+ * its epilogue.  No counterpart in the reference.  For every slot as there, with v[r] = float(sum_k a[f / top_k, k] *
+ * b[e, r, k]) * fl32(alpha_row[f / top_k] * alpha_col[e, r]) + bias[e, r]:
+ *     out[f, n] = act(v[n]) * v[N + n]
+ * in fp32, rounded once to out_dtype.  Rows of `out` that no slot names are left untouched, and so are those of blocks
+ * whose expert is not in [0, E).
+ *
+ *   b, alpha_col, bias   [E, 2 N, K], [E, 2 N] and NULL or [E, 2 N], contiguous: an expert's N rows inside the activation, then
+ *                        the N rows that its value multiplies
+ *   out                  [M * top_k, N] f16 or bf16, ldo
+ *   everything else, the workspace included, as for fnn_fused_moe_a8w8
+ */
+int fnn_fused_moe_a8w8_gated(const int8_t* a, int64_t lda, const int8_t* b, int64_t E, int64_t N, int64_t K,
+                             const void* alpha_row, int row_dtype, const void* alpha_col, int col_dtype, const void* bias,
+                             int bias_dtype, int activation, const int32_t* sorted_token_ids, int64_t EM,
+                             const int32_t* expert_ids, const int32_t* num_tokens_post_padded, int64_t num_valid_tokens,
+                             int top_k, int block_m, void* out, int out_dtype, int64_t ldo, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Routing of tokens to experts.  No counterpart in the reference.  Per token, with x its logits:
+ *     score[e] = softmax(x)[e] or sigmoid(x[e])
+ *     key[e]   = score[e] + bias[e]; without a bias score[e], compared as x[e] (both scores grow with the logit) unless
+ *                groups are compared by the sum of two of them
+ *     groups   (num_groups > 1) of E / num_groups consecutive experts: the topk_groups with the best group score stay, the largest
+ *              key of the group or the sum of its two largest
+ *     ids      the top_k experts with the largest keys among them, in that order
+ *     weights  score[ids], divided by their sum if renormalize, times scale
+ * The order is that of 64-bit arithmetic, equal keys go to the lowest index.  A NaN key ranks last, with the -infinities.  A
+ * row of -infinity logits has the weights 0 under the softmax.
+ *
+ *   logits        [M, E]  f16, bf16 or f32, ldl;  E at most 1024
+ *   bias          NULL or [E] f32
+ *   num_groups    a divisor of E, at most 32;  top_k at most 32 and at most topk_groups * E / num_groups
+ *   topk_weights  [M, top_k] f32;  topk_ids [M, top_k] int32, contiguous
+ */
+int fnn_moe_route(const void* logits, int logits_dtype, int64_t ldl, int64_t M, int64_t E, const float* bias, int scoring,
+                  int renormalize, int num_groups, int topk_groups, int group_score, float scale, int top_k,
+                  float* topk_weights, int32_t* topk_ids, void* stream);
+
+/*
+ * The slot list that the expert products read: the flat (token * top_k + choice) indices of topk_ids, grouped by expert
+ * in ascending order, every expert's group padded to a multiple of block_m with the value num_choices.  Experts are those in
+ * [first_expert, first_expert + E), numbered from 0 in expert_ids; a choice of any other expert (on another device, or
+ * dropped) gets no slot.  Slots behind the last block in use hold num_choices, their blocks expert 0.  No counterpart in the reference.
+ *
+ *   topk_ids          [num_choices] int32
+ *   sorted_token_ids  [EM] int32, EM = fnn_moe_sort_slots(num_choices, E, block_m): the most that any choice of experts fills
+ *   expert_ids        [EM / block_m] int32;  num_tokens_post_padded [1] int32 (device memory): slots in use
+ *   E                 at most 1024
+ */
+int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_t E, int64_t first_expert, int block_m,
+                 int32_t* sorted_token_ids, int64_t EM, int32_t* expert_ids, int32_t* num_tokens_post_padded, void* stream);
+int64_t fnn_moe_sort_slots(int64_t num_choices, int64_t E, int block_m);
+
+/*
+ * Sum over a token's choices:  out[m, n] = sum_j topk_weights[m, j] * c[m, j, n] + residual[m, n], summed in fp32 and rounded
+ * once.  No counterpart in the reference.
+ *
+ *   c             [M, top_k, N] f16 or bf16 (dtype), ldc_m and ldc_k elements between tokens and between choices
+ *   topk_weights  NULL (all 1, the expert products have applied them) or [M, top_k] f32, contiguous
+ *   topk_ids      NULL or [M, top_k] int32, contiguous: choices of experts outside [first_expert, first_expert + E) are left out,
+ *                 and their rows of c, which nothing has written, are not read
+ *   residual      NULL or [M, N] in dtype, ldr (0: the same row for every m);  it may be `out` itself (same pointer, ldr == ldo)
+ *   out           [M, N] in dtype, ldo
+ */
+int fnn_moe_combine(const void* c, int dtype, int64_t ldc_m, int64_t ldc_k, int64_t M, int64_t top_k, int64_t N,
+                    const float* topk_weights, const int32_t* topk_ids, int64_t E, int64_t first_expert,
+                    const void* residual, int64_t ldr, void* out, int64_t ldo, void* stream);
 
 /*
  * Fused mixture-of-experts weight-only GEMM over expert-sorted token slots, packed-int4 expert weights.

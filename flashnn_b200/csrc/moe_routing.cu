@@ -31,6 +31,7 @@ struct RouteParams {
   int M, E, top_k, groups, topk_groups, group_size;
   int softmax, renormalize, summed;  // summed: a group's score is the sum of its two largest keys, else its largest
   float scale;
+  int wide, wide_bias, slow_groups;  // set by the launch: lanes read whole words; groups that are not a power of two of lanes
 };
 
 // order-preserving map of keys to unsigned integers; a NaN ranks with -infinity, 0 is left for "not there"
@@ -55,12 +56,9 @@ template <> struct Ord<double> { using type = unsigned long long; };
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = u > v ? u : v;
-  }
-  return v;
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
+  return (static_cast<unsigned long long>(hi) << 32) | lo;
 }
 template <typename F> __device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
@@ -202,40 +200,256 @@ __device__ bool route_row(const float (&x)[PER], int lane, const RouteParams& p,
 
 constexpr int kRouteWarps = 8;
 
+// A lane's PER logits, experts lane * PER .. lane * PER + PER - 1; absent ones read as 0.
 template <typename T, int PER>
-__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(const RouteParams p) {
-  const int row = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
-  if (row >= p.M) return;
-  const int lane = threadIdx.x & 31;
-  const T* src = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
-  float x[PER];
+__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, bool wide, float (&x)[PER]) {
+  const T* src = reinterpret_cast<const T*>(p.logits) + row * p.ldl + lane * PER;
+  constexpr int kWord = 16 / int(sizeof(T)) < PER ? 16 / int(sizeof(T)) : PER;  // logits per load
+  if (wide) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) x[j] = lane * PER + j < p.E ? to_f32(src[lane * PER + j]) : 0.f;
+    for (int w = 0; w < PER / kWord; ++w) {
+      struct alignas(kWord * sizeof(T)) Word { T v[kWord]; };
+      Word u{};
+      if (lane * PER + w * kWord < p.E) u = *reinterpret_cast<const Word*>(src + w * kWord);
+#pragma unroll
+      for (int j = 0; j < kWord; ++j) x[w * kWord + j] = to_f32(u.v[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = lane * PER + j < p.E ? to_f32(src[j]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void write_choice(const RouteParams& p, int64_t row, int lane, int id, float score) {
+  if (lane < p.top_k) {
+    p.weights[row * p.top_k + lane] = score;
+    p.ids[row * p.top_k + lane] = id;
+  }
+}
+
+// Any row: round by round, in fp32 where that decides, else in 64 bits.  Kept out of line so that the registers of the
+// 64-bit form are not the fast kernel's.
+template <typename T, int PER>
+__device__ __noinline__ void route_slowly(const RouteParams& p, int64_t row, int lane, bool try_fp32) {
+  float x[PER];
+  load_logits<T, PER>(p, row, lane, false, x);
   int id = 0;
   float score = 0.f;
-  if (!route_row<float, PER>(x, lane, p, id, score)) {  // (the whole warp agrees)
+  if (!try_fp32 || !route_row<float, PER>(x, lane, p, id, score)) {  // (the whole warp agrees)
     double exact = 0.0;
     route_row<double, PER>(x, lane, p, id, exact);
     score = float(exact);
   }
-  if (lane < p.top_k) {
-    const int64_t at = int64_t(row) * p.top_k + lane;
-    p.weights[at] = score;
-    p.ids[at] = id;
+  write_choice(p, row, lane, id, score);
+}
+
+__device__ __forceinline__ float rcp_f32(float v) {  // within 1 unit in the last place
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_max_f32(float v) {  // (skips NaNs)
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The usual row.  A NaN marks what is not there (maxima skip it, comparisons with it are false).
+//
+// The top_k-th largest of the 32 lanes' largest keys is no larger than the top_k-th largest key, so the keys that are not
+// below it (by more than the tolerance) hold all that can be chosen; they are few, 12 or so for 8 of 256.  They move to one per lane, each
+// counts those before it, and that is its place.  Against top_k rounds of a maximum over the row this is a third of the
+// instructions, and instructions are what bounds it (a row of 256 fp32 logits is 1 KB of reads).
+// Rows with more than 32 such keys, with group shapes that are not whole powers of two of lanes, or that fp32 does not decide
+// go round by round.
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32, 4) moe_route_kernel(const __grid_constant__ RouteParams p) {
+  __shared__ float2 s_key[kRouteWarps][33];  // key and logit of the candidates, then of the choices in order
+  __shared__ int s_id[kRouteWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * kRouteWarps + warp;
+  if (row >= p.M) return;
+  if (p.slow_groups) return route_slowly<T, PER>(p, row, lane, true);
+  const float inf = __int_as_float(0x7f800000), nan = __int_as_float(0x7fffffff);
+  const int e0 = lane * PER;
+  const bool by_logit = p.bias == nullptr && !p.summed;
+  float x[PER];
+  load_logits<T, PER>(p, row, lane, p.wide, x);
+
+  // keys
+  float key[PER];
+  float top = 0.f, share = 1.f;  // softmax: score = exp(x - top) * share
+  if (p.softmax) {
+    top = -inf;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) top = fmaxf(top, e0 + j < p.E ? x[j] : -inf);
+    top = warp_max_f32(top);
+    if (top == inf || top == -inf) top = 0.f;
+    float total = 0.f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      key[j] = __expf(x[j] - top);
+      total += e0 + j < p.E ? key[j] : 0.f;
+    }
+    total = warp_sum(total);
+    share = total == 0.f ? 1.f : rcp_f32(total);
   }
+  if (by_logit) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = x[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = p.softmax ? key[j] * share : rcp_f32(1.f + __expf(-x[j]));
+    if (p.bias) {
+      if (PER >= 4 && p.wide_bias) {
+        if (e0 < p.E) {
+#pragma unroll
+          for (int j = 0; j < PER; j += 4) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + e0 + j));
+            key[j] += b.x;
+            if (PER >= 4) { key[j + 1 < PER ? j + 1 : 0] += b.y; key[j + 2 < PER ? j + 2 : 0] += b.z; key[j + 3 < PER ? j + 3 : 0] += b.w; }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (e0 + j < p.E) key[j] += __ldg(p.bias + e0 + j);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) key[j] = e0 + j < p.E ? fmaxf(key[j], -inf) : nan;  // (a NaN key ranks with -infinity)
+  // How far a key can be off: `off` plus `rel` of its size.  The hardware exponential adds as much to the softmax as the
+  // argument's rounding does (route_row): 260 * 2^-24 of a score, which is at most `share`, the best one's.  A sigmoid p of x is off
+  // by p (1 - p) (|x| + 4) + 4 p roundings of 2^-24, at most 5.4 of them.
+  const float off = by_logit ? 0.f : (p.softmax ? 1.6e-5f * share : 1e-6f) + 1e-37f;
+  const float rel = by_logit ? 0.f : 2.4e-7f;
+  bool sure = true;
+
+  bool in = e0 < p.E;
+  if (p.groups > 1) {
+    const int lanes = p.group_size / PER, g = lane / lanes;  // (whole groups of lanes, checked on the host)
+    float a = -inf, b = -inf;  // the group's two largest keys
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      b = fmaxf(b, fminf(a, key[j]));
+      a = fmaxf(a, key[j]);
+    }
+    for (int o = 1; o < lanes; o <<= 1) {
+      const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+      b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+      a = fmaxf(a, a2);
+    }
+    const bool two = p.summed && p.group_size > 1;
+    const float value = two ? fmaxf(a + b, -inf) : a;
+    int rank = 0;
+    for (int h = 0; h < p.groups; ++h) {
+      const float other = __shfl_sync(0xffffffffu, value, h * lanes);
+      rank += (other > value || (other == value && h < g)) ? 1 : 0;
+    }
+    const bool chosen = rank < p.topk_groups;
+    if (!by_logit && p.topk_groups < p.groups) {
+      const float slack = 2.f * off + rel * (fabsf(a) + (two ? fabsf(b) : 0.f) + fabsf(value));
+      const float worst_in = -warp_max_f32(in && chosen ? slack - value : -inf);  // what the worst in and the best out can be
+      const float best_out = warp_max_f32(in && !chosen ? value + slack : -inf);
+      if (!(worst_in > best_out)) sure = false;
+    }
+    in = in && chosen;
+  }
+
+  // a bound from below on the top_k-th largest key
+  float lane_top = nan;
+  if (in) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) lane_top = fmaxf(lane_top, key[j]);
+  }
+  float floor_key = -inf;
+  for (int i = 0; i < p.top_k; ++i) {
+    const float m = warp_max_f32(lane_top);
+    floor_key = m;
+    if (m != m) break;  // fewer lanes than choices: every key that is there
+    const uint32_t at = __ballot_sync(0xffffffffu, lane_top == m);
+    if (lane == __ffs(at) - 1) lane_top = nan;
+  }
+  if (!by_logit) floor_key -= 2.1f * (off + rel * fabsf(floor_key));
+  if (floor_key != floor_key) floor_key = -inf;  // (also -infinity less its own size)
+  // the keys that are not below it, one per lane
+  uint32_t picked = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) picked |= (in && key[j] >= floor_key) ? 1u << j : 0u;
+  const int mine = __popc(picked);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  const int count = __shfl_sync(0xffffffffu, upto, 31);
+  if (count > 32) return route_slowly<T, PER>(p, row, lane, true);
+  int at = upto - mine;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if ((picked >> j) & 1u) {
+      s_key[warp][at] = make_float2(key[j], x[j]);
+      s_id[warp][at] = e0 + j;
+      ++at;
+    }
+  }
+  __syncwarp();
+  const float2 kx = lane < count ? s_key[warp][lane] : make_float2(0.f, 0.f);
+  const int id = lane < count ? s_id[warp][lane] : 0;
+  const float k = kx.x;
+  int rank = 0;  // list order is expert order: equal keys keep it
+  for (int t = 0; t < count; ++t) {
+    const float other = __shfl_sync(0xffffffffu, k, t);
+    rank += (other > k || (other == k && t < lane)) ? 1 : 0;
+  }
+  __syncwarp();
+  if (lane < count) {
+    s_key[warp][rank] = kx;
+    s_id[warp][rank] = id;
+  }
+  __syncwarp();
+  const bool chosen = lane < p.top_k;
+  const int best = chosen ? s_id[warp][lane] : 0;
+  const float2 bx = chosen ? s_key[warp][lane] : make_float2(0.f, 0.f);
+  if (!by_logit && chosen && lane + 1 < count) {
+    const float next = s_key[warp][lane + 1].x;
+    if (!(bx.x - next > 2.f * off + rel * (fabsf(bx.x) + fabsf(next)))) sure = false;
+  }
+  // the scores of the chosen alone, with the exponential that is right to two units in the last place
+  float sc = p.softmax ? expf(bx.y - top) * share : __fdividef(1.f, 1.f + expf(-bx.y));
+  if (p.renormalize) {
+    float total = warp_sum(chosen ? sc : 0.f);
+    if (total < 1e-30f) sure = false;  // scores that fp32 cannot hold
+    sc = __fdiv_rn(sc, total);
+  }
+  if (!__all_sync(0xffffffffu, sure)) return route_slowly<T, PER>(p, row, lane, false);
+  write_choice(p, row, lane, best, sc * p.scale);
+}
+
+template <typename T, int PER>
+int launch_route_per(RouteParams p, cudaStream_t st) {
+  const unsigned grid = unsigned((int64_t(p.M) + kRouteWarps - 1) / kRouteWarps);
+  // lanes read whole words where every row starts on one and a lane has all of its experts or none
+  const int word = PER * int(sizeof(T)) < 16 ? PER * int(sizeof(T)) : 16;
+  p.wide = p.E % PER == 0 && reinterpret_cast<uintptr_t>(p.logits) % word == 0 && (p.ldl * int64_t(sizeof(T))) % word == 0;
+  p.wide_bias = p.E % PER == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+  const int lanes = p.group_size / PER;
+  p.slow_groups = p.groups > 1 && (p.group_size % PER != 0 || (lanes & (lanes - 1)) != 0);
+  moe_route_kernel<T, PER><<<grid, kRouteWarps * 32, 0, st>>>(p);
+  return check_cuda(cudaGetLastError(), "moe_route launch");
 }
 
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t st) {
-  const unsigned grid = unsigned((p.M + kRouteWarps - 1) / kRouteWarps);
   const int per = (p.E + 31) / 32;
-  if (per <= 1) moe_route_kernel<T, 1><<<grid, kRouteWarps * 32, 0, st>>>(p);
-  else if (per <= 2) moe_route_kernel<T, 2><<<grid, kRouteWarps * 32, 0, st>>>(p);
-  else if (per <= 4) moe_route_kernel<T, 4><<<grid, kRouteWarps * 32, 0, st>>>(p);
-  else if (per <= 8) moe_route_kernel<T, 8><<<grid, kRouteWarps * 32, 0, st>>>(p);
-  else if (per <= 16) moe_route_kernel<T, 16><<<grid, kRouteWarps * 32, 0, st>>>(p);
-  else moe_route_kernel<T, 32><<<grid, kRouteWarps * 32, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "moe_route launch");
+  if (per <= 1) return launch_route_per<T, 1>(p, st);
+  if (per <= 2) return launch_route_per<T, 2>(p, st);
+  if (per <= 4) return launch_route_per<T, 4>(p, st);
+  if (per <= 8) return launch_route_per<T, 8>(p, st);
+  if (per <= 16) return launch_route_per<T, 16>(p, st);
+  return launch_route_per<T, 32>(p, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -244,10 +458,13 @@ int launch_route(const RouteParams& p, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // One cluster does it in one launch.  Its warps take consecutive pieces of the list.  Pass 1 counts each warp's experts in
 // shared memory; prefix sums over a CTA's warps, over the cluster's CTAs (through distributed shared memory) and over the
-// experts' padded sizes give every warp its first slot of every expert; pass 2 hands the slots out in list order (a match
-// over the warp ranks equal experts).  No atomics decide an order: the list is the same every time.
+// experts' padded sizes give every warp its first slot of every expert; pass 2 hands the slots out in list order.  A vote
+// per bit of the expert ranks equal ones within a warp: match.any takes about 100 cycles for 32 different values, and with it the
+// list of 131072 choices took 25 us, ... with votes.  No atomics decide an order: the list is the same every time.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kHeld = 16;
+constexpr unsigned kNoExpert = 0xffffffffu;
 constexpr int kSortMaxExperts = 1024;  // one thread per expert in the prefix sums
 
 struct SortParams {
@@ -263,6 +480,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   int32_t* total = cnt + kSortWarps * p.E;    // [E] this CTA's counts
   int32_t* begin = total + p.E;               // [E] first slot of the expert
   int32_t* count = begin + p.E;               // [E] slots in use of the expert
+  int32_t* base = count + p.E;                // [E] first slot of the expert that is this CTA's
   __shared__ int32_t scan[kSortWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = int(cluster.block_rank()), ctas = int(cluster.num_blocks());
@@ -274,20 +492,34 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   const int hi = int(lo64 + piece < p.choices ? lo64 + piece : p.choices);
   int32_t* mine = cnt + warp * p.E;
 
+  // experts of the piece's first kHeld steps stay in registers between the passes (all of it up to 131072 choices on eight CTAs)
+  auto expert_of = [&](int i) {
+    const unsigned x = i < hi ? unsigned(__ldg(p.ids + i)) - unsigned(p.first) : kNoExpert;
+    return x < unsigned(p.E) ? x : kNoExpert;
+  };
+  unsigned held[kHeld];
+#pragma unroll
+  for (int s = 0; s < kHeld; ++s) held[s] = expert_of(lo + s * 32 + lane);
   for (int i = threadIdx.x; i < kSortWarps * p.E; i += kSortThreads) cnt[i] = 0;
   __syncthreads();
-  for (int i = lo + lane; i < hi; i += 32) {
-    const unsigned e = unsigned(p.ids[i]) - unsigned(p.first);
-    if (e < unsigned(p.E)) atomicAdd(mine + e, 1);
+#pragma unroll
+  for (int s = 0; s < kHeld; ++s)
+    if (held[s] != kNoExpert) atomicAdd(mine + held[s], 1);
+  for (int i = lo + kHeld * 32 + lane; i < hi; i += 32) {
+    const unsigned x = expert_of(i);
+    if (x != kNoExpert) atomicAdd(mine + x, 1);
   }
   __syncthreads();
   const int e = threadIdx.x;
   if (e < p.E) {
+    int t[kSortWarps];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) t[w] = cnt[w * p.E + e];
     int run = 0;
+#pragma unroll
     for (int w = 0; w < kSortWarps; ++w) {
-      const int t = cnt[w * p.E + e];
       cnt[w * p.E + e] = run;
-      run += t;
+      run += t[w];
     }
     total[e] = run;
   }
@@ -324,24 +556,31 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   if (e < p.E) {
     begin[e] = start;
     count[e] = all;
-    for (int w = 0; w < kSortWarps; ++w) cnt[w * p.E + e] += start + before;
+    base[e] = start + before;
   }
   if (rank == 0 && threadIdx.x == 0) *p.num_post_padded = in_use;
   __syncthreads();
 
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    unsigned ex = i < hi ? unsigned(p.ids[i]) - unsigned(p.first) : 0xffffffffu;
-    if (ex >= unsigned(p.E)) ex = 0xffffffffu;
-    const uint32_t same = __match_any_sync(0xffffffffu, ex);
-    const bool here = ex != 0xffffffffu;
-    const int base = here ? mine[ex] : 0;
+  const int bits = 32 - __clz(p.E - 1 > 0 ? p.E - 1 : 0);
+  auto hand_out = [&](unsigned x, int i) {
+    const bool here = x != kNoExpert;
+    uint32_t same = __ballot_sync(0xffffffffu, here);
+    for (int b = 0; b < bits; ++b) {
+      const uint32_t one = __ballot_sync(0xffffffffu, (x >> b) & 1u);
+      same &= ((x >> b) & 1u) ? one : ~one;
+    }
     const int ahead = __popc(same & ((1u << lane) - 1u));
+    int next = 0;
+    if (here) next = mine[x];
     __syncwarp();
-    if (here && ahead == 0) mine[ex] = base + __popc(same);
+    if (here && ahead == 0) mine[x] = next + __popc(same);
     __syncwarp();
-    if (here) p.sorted[base + ahead] = i;
-  }
+    if (here) p.sorted[base[x] + next + ahead] = i;
+  };
+#pragma unroll
+  for (int s = 0; s < kHeld; ++s)
+    if (lo + s * 32 < hi) hand_out(held[s], lo + s * 32 + lane);
+  for (int i = lo + kHeld * 32; i < hi; i += 32) hand_out(expert_of(i + lane), i + lane);
   // padding slots and the blocks' experts
   for (int x = gw; x < p.E; x += warps) {
     const int b = begin[x], n = count[x], end = b + (n + p.bm - 1) / p.bm * p.bm;
@@ -466,14 +705,14 @@ extern "C" int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_
   if (!num_tokens_post_padded || (num_choices > 0 && (!topk_ids || !sorted_token_ids || !expert_ids)))
     return fail(FNN_ERR_NULL_POINTER, "moe_sort: null tensor pointer");
   SortParams p{topk_ids, sorted_token_ids, expert_ids, num_tokens_post_padded, int(num_choices), int(E), block_m, int(first_expert), int(EM)};
-  const size_t smem = size_t(kSortWarps + 3) * size_t(E) * sizeof(int32_t);
+  const size_t smem = size_t(kSortWarps + 4) * size_t(E) * sizeof(int32_t);
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
   cudaGetDevice(&dev);
   dev &= 63;
   std::call_once(once[dev], [&] {
-    attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortWarps + 3) * kSortMaxExperts * 4);
+    attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortWarps + 4) * kSortMaxExperts * 4);
   });
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(moe_sort)");
   cudaLaunchConfig_t cfg = {};

@@ -42,8 +42,8 @@ class MoeRouting(BackendKernel):
         if bias is not None:
             assert bias.numel() == e and bias.is_floating_point(), "bias must be [num_experts]"
             bias = bias.reshape(-1).to(torch.float32).contiguous()
-        weights = torch.empty((m, self.top_k), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((m, self.top_k), dtype=torch.int32, device=logits.device)
+        weights = logits.new_empty((m, self.top_k), dtype=torch.float32)
+        ids = logits.new_empty((m, self.top_k), dtype=torch.int32)
         with _on_device(logits):
             _lib.check(_lib.lib().fnn_moe_route(
                 logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if m > 1 else e, m, e,
@@ -69,9 +69,8 @@ def moe_sort_tokens(topk_ids, num_experts, BM, first_expert=0):
     ids = _i32(topk_ids).contiguous()
     L = _lib.lib()
     em = L.fnn_moe_sort_slots(ids.numel(), num_experts, BM)
-    sorted_ids = torch.empty(em, dtype=torch.int32, device=ids.device)
-    experts = torch.empty(em // BM, dtype=torch.int32, device=ids.device)
-    in_use = torch.empty(1, dtype=torch.int32, device=ids.device)
+    # one allocation, three views
+    sorted_ids, experts, in_use = ids.new_empty(em + em // BM + 1).split((em, em // BM, 1))
     with _on_device(ids):
         _lib.check(L.fnn_moe_sort(ids.data_ptr(), ids.numel(), num_experts, first_expert, BM, sorted_ids.data_ptr(), em,
                                   experts.data_ptr(), in_use.data_ptr(), _stream(ids)))
@@ -101,7 +100,7 @@ def moe_combine(C, topk_weights=None, topk_ids=None, num_experts=None, first_exp
         if n > 1 and residual.stride(1) != 1:
             residual = residual.contiguous()
         ldr = residual.stride(0) if m > 1 else n
-    out = torch.empty((m, n), dtype=C.dtype, device=C.device)
+    out = C.new_empty((m, n))
     with _on_device(C):
         _lib.check(_lib.lib().fnn_moe_combine(
             C.data_ptr(), _DT[C.dtype], C.stride(0) if m > 1 else k * n, C.stride(1) if k > 1 else n, m, k, n,

@@ -3,6 +3,7 @@
 #include <cooperative_groups.h>
 
 #include <mutex>
+#include <utility>
 
 #include "common.cuh"
 #include "quantise.cuh"
@@ -15,13 +16,17 @@ namespace {
 // ---------------------------------------------------------------------------
 // Routing: scores, balancing bias, group-limited choice, top-k, renormalised weights
 // ---------------------------------------------------------------------------
-// One warp per token, the row in registers: lane l holds experts l * PER .. l * PER + PER - 1, so that lane order is expert
-// order and the lowest lane among equals holds the lowest expert.
+// General form, one warp per token, the row in registers: lane l holds experts l * PER .. l * PER + PER - 1, so that lane order is
+// expert order and the lowest lane among equals holds the lowest expert.  Every lane sorts its keys (an odd-even merge network of
+// minima and maxima, without the experts' numbers), and top_k rounds take the largest of the 32 heads; the lane it came from
+// moves on to its next key.  A choice's expert is found afterwards, as the place of its value among that lane's unsorted keys.
+// Instructions bound the kernel (a row of 256 fp32 logits is 1 KB of reads).
 //
 // Which experts are chosen, and in what order, is defined in 64 bits.  Where the keys are the logits themselves (no bias,
 // no sum over a group: both scores grow with the logit) comparing them is exact.  Elsewhere the row is done in fp32 first,
 // with a bound on how far a key can be off; only where two keys that decide something are nearer than that (a row in some
-// hundreds) is the row done again in 64 bits.
+// hundreds) is the row done again in 64 bits, after the warp's others, so that the registers of the 64-bit form are not the
+// usual row's.
 struct RouteParams {
   const void* logits;
   const float* bias;  // nullptr or [E]
@@ -31,188 +36,119 @@ struct RouteParams {
   int M, E, top_k, groups, topk_groups, group_size;
   int softmax, renormalize, summed;  // summed: a group's score is the sum of its two largest keys, else its largest
   float scale;
-  int wide, wide_bias, slow_groups;  // set by the launch: lanes read whole words; groups that are not a power of two of lanes
+  int wide;        // lanes read whole words (set by the launch)
+  int whole_lanes; // a group is a power of two of lanes with all of their experts (set by the launch)
 };
 
-// order-preserving map of keys to unsigned integers; a NaN ranks with -infinity, 0 is left for "not there"
-__device__ __forceinline__ uint32_t ordered(float v) {
-  v = v != v ? __int_as_float(0xff800000) : v + 0.f;  // (-0 -> +0)
-  const uint32_t b = __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+// maxima and minima that skip a NaN, which marks what is not there
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
-__device__ __forceinline__ unsigned long long ordered(double v) {
-  v = v != v ? __longlong_as_double(0xfff0000000000000ll) : v + 0.0;
-  const unsigned long long b = __double_as_longlong(v);
-  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
-}
-__device__ __forceinline__ float from_ordered(uint32_t o) {
-  return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
-}
-__device__ __forceinline__ double from_ordered(unsigned long long o) {
+__device__ __forceinline__ double warp_max(double v) {
+  // order-preserving map to unsigned integers, 0 for a NaN; the upper words' maximum, then the lower words' among those
+  v += 0.0;  // (-0 -> +0)
+  unsigned long long o = __double_as_longlong(v);
+  o = v != v ? 0ull : (o >> 63) ? ~o : o | 0x8000000000000000ull;
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(o >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(o >> 32) == hi ? uint32_t(o) : 0u);
+  o = (static_cast<unsigned long long>(hi) << 32) | lo;
+  if (o == 0ull) return __longlong_as_double(0x7fffffffffffffffll);
   return __longlong_as_double((o >> 63) ? o & 0x7fffffffffffffffull : ~o);
-}
-template <typename F> struct Ord { using type = uint32_t; };
-template <> struct Ord<double> { using type = unsigned long long; };
-
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ unsigned long long warp_max(unsigned long long v) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(v >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
-  return (static_cast<unsigned long long>(hi) << 32) | lo;
 }
 template <typename F> __device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+// e^v of the keys: in fp32 by the hardware's 2^v, within (|v| + 4) roundings of 2^-24, 0 where that is subnormal
+__device__ __forceinline__ float key_exp(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ double key_exp(double v) { return exp(v); }
+__device__ __forceinline__ float reciprocal(float v) {  // within 1 unit in the last place
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
+__device__ __forceinline__ float full_exp(float v) { return expf(v); }
+__device__ __forceinline__ double full_exp(double v) { return exp(v); }
 
-// One row in arithmetic F.  Lane i < top_k receives the i-th choice and its score; returns false where fp32 does not decide.
-template <typename F, int PER>
-__device__ bool route_row(const float (&x)[PER], int lane, const RouteParams& p, int& id, F& score) {
-  using O = typename Ord<F>::type;
-  constexpr bool kExact = sizeof(F) == 8;
-  const F inf = F(__int_as_float(0x7f800000));
-  const int e0 = lane * PER;
-  const bool by_logit = p.bias == nullptr && !p.summed;
-  // scores
-  F s[PER];
-  F widest = F(0);  // largest |key| or score of the row
-  if (p.softmax) {
-    O top_o = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (e0 + j < p.E) top_o = max(top_o, ordered(F(x[j])));
-    F top = from_ordered(warp_max(top_o));
-    if (top == inf || top == -inf) top = F(0);
-    F total = F(0);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      s[j] = e0 + j < p.E ? exp_of(F(x[j]) - top) : F(0);
-      total += s[j];
-    }
-    total = warp_sum(total);
-    if (total == F(0)) total = F(1);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] /= total;
-  } else {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] = F(1) / (F(1) + exp_of(-F(x[j])));
+// odd-even merge network: with runs of P sorted, partners K apart within runs of 2 P
+template <int P, int K, int I, typename F, int N> __device__ __forceinline__ void compare_exchange(F (&v)[N]) {
+  if constexpr (I + K < N && I >= K % P && ((I - K % P) / K) % 2 == 0 && I / (2 * P) == (I + K) / (2 * P)) {
+    const F a = larger(v[I], v[I + K]), b = smaller(v[I], v[I + K]);
+    v[I] = a;
+    v[I + K] = b;
   }
-  // keys
-  O key[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    F k = F(x[j]);
-    if (!by_logit) {
-      k = s[j];
-      if (p.bias && e0 + j < p.E) k += F(__ldg(p.bias + e0 + j));
-    }
-    key[j] = e0 + j < p.E ? ordered(k) : O(0);
-    if (!kExact && !by_logit && e0 + j < p.E) {
-      const F a = fmaxf(fabsf(k), s[j]);
-      if (a < inf) widest = fmaxf(widest, a);
-    }
+}
+template <int P, int K, typename F, int N, int... I>
+__device__ __forceinline__ void merge_step(F (&v)[N], std::integer_sequence<int, I...>) {
+  (compare_exchange<P, K, I>(v), ...);
+}
+template <int P, int K, typename F, int N> __device__ __forceinline__ void merge_runs(F (&v)[N]) {
+  merge_step<P, K>(v, std::make_integer_sequence<int, N>());
+  if constexpr (K > 1) merge_runs<P, K / 2>(v);
+}
+template <int P = 1, typename F, int N> __device__ __forceinline__ void sort_descending(F (&v)[N]) {
+  if constexpr (P < N) {
+    merge_runs<P, P>(v);
+    sort_descending<2 * P>(v);
   }
-  // How far an fp32 key can be off.  The sigmoid is within 4 roundings (2^-24 of its value each).  The softmax's argument x - max
-  // is rounded by 2^-24 of up to 104 (beyond that the result is 0), its sum by one rounding per addition (at most
-  // 37 in a row); its exponential and the division take 4 more: below 2^-16 of the value.  Adding the bias rounds once more.
-  F tol = F(0);
-  if (!kExact && !by_logit) tol = from_ordered(warp_max(ordered(widest))) * (p.softmax ? F(1.6e-5f) : F(5e-7f)) + F(1e-37f);
-  bool sure = true;
-
-  if (p.groups > 1) {
-    // lane g < groups: the score of group g
-    O mine = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const int lo = g * p.group_size, hi = lo + p.group_size;
-      O best = 0;
-      int at = -1;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (e0 + j >= lo && e0 + j < hi && key[j] > best) { best = key[j]; at = j; }
-      const O first = warp_max(best);
-      O value = first;
-      if (p.summed && p.group_size > 1) {
-        const int src = __ffs(__ballot_sync(0xffffffffu, best == first)) - 1;
-        O second = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (e0 + j >= lo && e0 + j < hi && !(lane == src && j == at) && key[j] > second) second = key[j];
-        value = ordered(from_ordered(first) + from_ordered(warp_max(second)));
-      }
-      if (lane == g) mine = value;
-    }
-    // its rank: groups with a larger score, or an equal one and a lower index
-    int rank = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const O other = __shfl_sync(0xffffffffu, mine, g);
-      rank += (other > mine || (other == mine && g < lane)) ? 1 : 0;
-    }
-    const bool in = lane < p.groups && rank < p.topk_groups;
-    const uint32_t chosen = __ballot_sync(0xffffffffu, in);
-    if (!kExact && !by_logit && p.topk_groups < p.groups) {
-      const O worst_in = ~warp_max(in ? ~mine : O(0));
-      const O best_out = warp_max((lane < p.groups && !in) ? mine : O(0));
-      const F gap = from_ordered(worst_in) - from_ordered(best_out);
-      if (!(gap > F(4) * tol)) sure = false;  // (two keys each; also where both are infinite)
-    }
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (e0 + j < p.E && !((chosen >> ((e0 + j) / p.group_size)) & 1u)) key[j] = 0;
-  }
-
-  // the top_k largest keys in order
-  O last = 0;
-  const int rounds = (!kExact && !by_logit) ? p.top_k + 1 : p.top_k;  // one more shows how near the first one left out is
-  for (int i = 0; i < rounds; ++i) {
-    O best = 0;
-    int at = 0;
-    F sc = F(0);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (key[j] > best) { best = key[j]; at = j; sc = s[j]; }
-    const O m = warp_max(best);
-    if (m == 0) break;  // (only the extra round can find nothing)
-    if (!kExact && !by_logit && i > 0 && !(from_ordered(last) - from_ordered(m) > F(2) * tol)) sure = false;
-    last = m;
-    if (i == p.top_k) break;
-    const int src = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
-    const int expert = __shfl_sync(0xffffffffu, e0 + at, src);
-    const F value = __shfl_sync(0xffffffffu, sc, src);
-    if (lane == i) { id = expert; score = value; }
-    if (lane == src) {
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (j == at) key[j] = 0;
-    }
-  }
-  if (p.renormalize) {
-    F total = warp_sum(lane < p.top_k ? score : F(0));
-    if (!kExact && total < F(1e-30f)) sure = false;  // (scores that fp32 cannot hold)
-    if (total == F(0)) total = F(1);
-    score /= total;
-  }
-  score *= F(p.scale);
-  return sure;
 }
 
-constexpr int kRouteWarps = 8;
+// sorts a bitonic sequence
+template <int K, typename F, int N, int... I>
+__device__ __forceinline__ void bitonic_step(F (&v)[N], std::integer_sequence<int, I...>) {
+  auto one = [&](auto index) {
+    constexpr int i = decltype(index)::value;
+    if constexpr ((i & K) == 0) {
+      const F a = larger(v[i], v[i + K]), b = smaller(v[i], v[i + K]);
+      v[i] = a;
+      v[i + K] = b;
+    }
+  };
+  (one(std::integral_constant<int, I>()), ...);
+}
+template <int K, typename F, int N> __device__ __forceinline__ void merge_bitonic(F (&v)[N]) {
+  if constexpr (K >= 1) {
+    bitonic_step<K>(v, std::make_integer_sequence<int, N>());
+    merge_bitonic<K / 2>(v);
+  }
+}
 
-// A lane's PER logits, experts lane * PER .. lane * PER + PER - 1; absent ones read as 0.
+// A lane's PER logits; absent ones read as 0.
+template <typename T> __device__ __forceinline__ void load_word(const T* src, bool on, float (&x)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) v = *reinterpret_cast<const float4*>(src);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+    uint2 v = make_uint2(0u, 0u);
+    if (on) v = *reinterpret_cast<const uint2*>(src);
+    x[0] = lo_of<T>(v.x); x[1] = hi_of<T>(v.x); x[2] = lo_of<T>(v.y); x[3] = hi_of<T>(v.y);
+  }
+}
 template <typename T, int PER>
-__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, bool wide, float (&x)[PER]) {
+__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, float (&x)[PER]) {
   const T* src = reinterpret_cast<const T*>(p.logits) + row * p.ldl + lane * PER;
-  constexpr int kWord = 16 / int(sizeof(T)) < PER ? 16 / int(sizeof(T)) : PER;  // logits per load
-  if (wide) {
+  if (PER >= 4 && p.wide) {
+    const bool on = lane * PER < p.E;
 #pragma unroll
-    for (int w = 0; w < PER / kWord; ++w) {
-      struct alignas(kWord * sizeof(T)) Word { T v[kWord]; };
-      Word u{};
-      if (lane * PER + w * kWord < p.E) u = *reinterpret_cast<const Word*>(src + w * kWord);
+    for (int w = 0; w < PER; w += 4) {
+      float v[4];
+      load_word(src + w, on, v);
 #pragma unroll
-      for (int j = 0; j < kWord; ++j) x[w * kWord + j] = to_f32(u.v[j]);
+      for (int j = 0; j < 4; ++j)
+        if (w + j < PER) x[w + j] = v[j];
     }
   } else {
 #pragma unroll
@@ -220,229 +156,618 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, i
   }
 }
 
-__device__ __forceinline__ void write_choice(const RouteParams& p, int64_t row, int lane, int id, float score) {
-  if (lane < p.top_k) {
-    p.weights[row * p.top_k + lane] = score;
-    p.ids[row * p.top_k + lane] = id;
-  }
-}
-
-// Any row: round by round, in fp32 where that decides, else in 64 bits.  Kept out of line so that the registers of the
-// 64-bit form are not the fast kernel's.
-template <typename T, int PER>
-__device__ __noinline__ void route_slowly(const RouteParams& p, int64_t row, int lane, bool try_fp32) {
-  float x[PER];
-  load_logits<T, PER>(p, row, lane, false, x);
-  int id = 0;
-  float score = 0.f;
-  if (!try_fp32 || !route_row<float, PER>(x, lane, p, id, score)) {  // (the whole warp agrees)
-    double exact = 0.0;
-    route_row<double, PER>(x, lane, p, id, exact);
-    score = float(exact);
-  }
-  write_choice(p, row, lane, id, score);
-}
-
-__device__ __forceinline__ float rcp_f32(float v) {  // within 1 unit in the last place
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float warp_max_f32(float v) {  // (skips NaNs)
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-// The usual row.  A NaN marks what is not there (maxima skip it, comparisons with it are false).
-//
-// The top_k-th largest of the 32 lanes' largest keys is no larger than the top_k-th largest key, so the keys that are not
-// below it (by more than the tolerance) hold all that can be chosen; they are few, 12 or so for 8 of 256.  They move to one per lane, each
-// counts those before it, and that is its place.  Against top_k rounds of a maximum over the row this is a third of the
-// instructions, and instructions are what bounds it (a row of 256 fp32 logits is 1 KB of reads).
-// Rows with more than 32 such keys, with group shapes that are not whole powers of two of lanes, or that fp32 does not decide
-// go round by round.
-template <typename T, int PER>
-__global__ void __launch_bounds__(kRouteWarps * 32, 4) moe_route_kernel(const __grid_constant__ RouteParams p) {
-  __shared__ float2 s_key[kRouteWarps][33];  // key and logit of the candidates, then of the choices in order
-  __shared__ int s_id[kRouteWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * kRouteWarps + warp;
-  if (row >= p.M) return;
-  if (p.slow_groups) return route_slowly<T, PER>(p, row, lane, true);
-  const float inf = __int_as_float(0x7f800000), nan = __int_as_float(0x7fffffff);
+// One row in arithmetic F; writes the choices, or returns false where fp32 does not decide.  s_bias: the biases in shared memory, 0
+// behind the last; s_keys: this warp's [PER][32] words of shared memory.
+template <typename F, typename T, int PER>
+__device__ __forceinline__ bool route_row(const RouteParams& p, const float (&x)[PER], int64_t row, int lane, const float* s_bias, F* s_keys) {
+  constexpr bool kExact = sizeof(F) == 8;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const F inf = F(__int_as_float(0x7f800000)), nan = F(__int_as_float(0x7fffffff));
   const int e0 = lane * PER;
   const bool by_logit = p.bias == nullptr && !p.summed;
-  float x[PER];
-  load_logits<T, PER>(p, row, lane, p.wide, x);
+  const bool check = !kExact && !by_logit;
+  // the lane's experts that can be chosen, one bit each
+  const int present = min(max(p.E - e0, 0), PER);
+  uint32_t real = present == 32 ? kAll : (1u << present) - 1u;
 
   // keys
-  float key[PER];
-  float top = 0.f, share = 1.f;  // softmax: score = exp(x - top) * share
+  F key[PER];
+  F top = F(0), share = F(1);  // softmax: score = exp(x - top) * share
   if (p.softmax) {
     top = -inf;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) top = fmaxf(top, e0 + j < p.E ? x[j] : -inf);
-    top = warp_max_f32(top);
-    if (top == inf || top == -inf) top = 0.f;
-    float total = 0.f;
+    for (int j = 0; j < PER; ++j) top = larger(top, j < present ? F(x[j]) : -inf);
+    top = warp_max(top);
+    if (top == inf || top == -inf) top = F(0);
+    F total = F(0);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      key[j] = __expf(x[j] - top);
-      total += e0 + j < p.E ? key[j] : 0.f;
+      key[j] = key_exp(F(x[j]) - top);
+      total += j < present ? key[j] : F(0);
     }
     total = warp_sum(total);
-    share = total == 0.f ? 1.f : rcp_f32(total);
+    share = total == F(0) ? F(1) : reciprocal(total);
+    if (!by_logit) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = kExact ? key[j] / (total == F(0) ? F(1) : total) : key[j] * share;
+    }
+  } else if (!by_logit) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = reciprocal(F(1) + key_exp(-F(x[j])));
   }
   if (by_logit) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = x[j];
-  } else {
+    for (int j = 0; j < PER; ++j) key[j] = F(x[j]);
+  } else if (p.bias) {
+    if constexpr (PER >= 4) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = p.softmax ? key[j] * share : rcp_f32(1.f + __expf(-x[j]));
-    if (p.bias) {
-      if (PER >= 4 && p.wide_bias) {
-        if (e0 < p.E) {
+      for (int j = 0; j < PER; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(s_bias + e0 + j);
+        key[j] += F(b.x); key[j + 1] += F(b.y); key[j + 2] += F(b.z); key[j + 3] += F(b.w);
+      }
+    } else {
 #pragma unroll
-          for (int j = 0; j < PER; j += 4) {
-            const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + e0 + j));
-            key[j] += b.x;
-            if (PER >= 4) { key[j + 1 < PER ? j + 1 : 0] += b.y; key[j + 2 < PER ? j + 2 : 0] += b.z; key[j + 3 < PER ? j + 3 : 0] += b.w; }
-          }
+      for (int j = 0; j < PER; ++j) key[j] += F(s_bias[e0 + j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) key[j] = j < present ? larger(key[j], -inf) : -inf;  // (a NaN key ranks with -infinity)
+  // How far an fp32 key can be off: `off` plus `rel` of its size.  A softmax score's argument is rounded by 2^-24 of up to 104
+  // (beyond that it is 0), the hardware exponential adds as much and the sum one rounding per addition (37 in a row): at most
+  // 2 * 104 + 50 roundings of 2^-24 of the score, which is at most `share`, the best one's.  A sigmoid q of x is off by
+  // q (1 - q) (|x| + 4) + 4 q such roundings, at most 5.4.
+  const F off = check ? (p.softmax ? F(1.6e-5f) * share : F(3.4e-7f)) + F(1e-37f) : F(0);
+  const F rel = check ? F(1.2e-7f) : F(0);
+  bool sure = true;
+
+  if (p.groups > 1) {
+    const bool two = p.summed && p.group_size > 1;
+    F a = -inf, b = -inf;  // the two largest keys: of this lane's group, or (below) of group `lane`
+    int g, lanes = 1;      // group h's are in lane h * lanes
+    if (p.whole_lanes) {
+      lanes = p.group_size / PER;
+      g = lane / lanes;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        b = larger(b, smaller(a, key[j]));
+        a = larger(a, key[j]);
+      }
+      for (int o = 1; o < lanes; o <<= 1) {
+        const F a2 = __shfl_xor_sync(kAll, a, o), b2 = __shfl_xor_sync(kAll, b, o);
+        b = larger(smaller(a, a2), larger(b, b2));
+        a = larger(a, a2);
+      }
+    } else {
+      g = lane;
+      for (int h = 0; h < p.groups; ++h) {
+        const int lo = h * p.group_size - e0, hi = lo + p.group_size;
+        F a1 = -inf, b1 = -inf;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const F v = j >= lo && j < hi ? key[j] : -inf;
+          b1 = larger(b1, smaller(a1, v));
+          a1 = larger(a1, v);
         }
-      } else {
+        const F first = warp_max(a1);
+        const int src = __ffs(__ballot_sync(kAll, a1 == first)) - 1;
+        const F second = warp_max(lane == src ? b1 : a1);
+        if (lane == h) { a = first; b = second; }
+      }
+    }
+    const F value = two ? larger(a + b, -inf) : a;
+    int rank = 0;
+#pragma unroll 4
+    for (int h = 0; h < p.groups; ++h) {
+      const F other = __shfl_sync(kAll, value, h * lanes);
+      rank += (other > value || (other == value && h < g)) ? 1 : 0;
+    }
+    const bool valid = g < p.groups, chosen = rank < p.topk_groups;
+    if (check && p.topk_groups < p.groups) {
+      const F slack = F(2) * off + rel * (fabsf(a) + (two ? fabsf(b) : F(0)) + fabsf(value));
+      const F worst_in = -warp_max(valid && chosen ? slack - value : -inf);  // what the worst in and the best out can be
+      const F best_out = warp_max(valid && !chosen ? value + slack : -inf);
+      if (!(worst_in > best_out)) sure = false;
+    }
+    if (p.whole_lanes) {
+      if (!chosen) real = 0;
+    } else {
+      const uint32_t in = __ballot_sync(kAll, valid && chosen);
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (e0 + j < p.E) key[j] += __ldg(p.bias + e0 + j);
+      for (int j = 0; j < PER; ++j)
+        if (j < present && !((in >> ((e0 + j) / p.group_size)) & 1u)) {
+          real &= ~(1u << j);
+          key[j] = -inf;
+        }
+    }
+  }
+
+  // rounds
+  F sorted[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) sorted[j] = key[j];
+  sort_descending(sorted);
+  const int mine = __popc(real);  // what cannot be chosen has sunk to the end
+  F* list = s_keys + lane;  // [PER][32]
+#pragma unroll
+  for (int j = 0; j < PER; ++j) list[j * 32] = sorted[j];
+  F head = mine > 0 ? sorted[0] : nan;
+  int at = 0;
+  F value = F(0);         // of this lane's choice (lane top_k: of the first one left out, which shows how near it is)
+  int from = 0;           // the lane it came from
+  F last = F(0);
+  bool repeated = false;  // two choices have the same key
+  bool extra = false;     // there is one left out
+  const int rounds = check ? p.top_k + 1 : p.top_k;
+  for (int i = 0; i < rounds; ++i) {
+    const F m = warp_max(head);
+    if (m != m) break;  // (only the extra round can find nothing)
+    extra = i == p.top_k;
+    const int src = __ffs(__ballot_sync(kAll, head == m)) - 1;
+    repeated |= i > 0 && m == last;
+    last = m;
+    value = lane == i ? m : value;
+    from = lane == i ? src : from;
+    at += lane == src ? 1 : 0;
+    const F next = list[min(at, PER - 1) * 32];
+    head = lane != src ? head : at < mine ? next : nan;
+  }
+  if (check) {
+    const F next = __shfl_down_sync(kAll, value, 1);
+    if (lane < p.top_k && (extra || lane + 1 < p.top_k) && !(value - next > F(2) * off + rel * (fabsf(value) + fabsf(next)))) sure = false;
+    if (!__all_sync(kAll, sure)) return false;
+  }
+
+  // the choice's expert: the first of that lane's experts with this key that no choice before it took
+  uint32_t equal = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) equal |= __shfl_sync(kAll, key[j], from) == value ? 1u << j : 0u;
+  equal &= __shfl_sync(kAll, real, from);
+  if (repeated) {
+    for (int i = 0; i + 1 < p.top_k; ++i) {
+      const F v = __shfl_sync(kAll, value, i);
+      const int src = __shfl_sync(kAll, from, i);
+      if (i < lane && v == value && src == from) equal &= equal - 1u;
+    }
+  }
+  const bool chosen = lane < p.top_k;
+  const int id = from * PER + (chosen ? __ffs(equal) - 1 : 0);
+  // the chosen ones' scores, with the full exponential
+  F score = F(0);
+  if (chosen) {
+    const F v = F(to_f32(reinterpret_cast<const T*>(p.logits)[row * p.ldl + id]));
+    score = p.softmax ? full_exp(v - top) * share : F(1) / (F(1) + full_exp(-v));
+  }
+  if (p.renormalize) {
+    F total = warp_sum(score);
+    if (!kExact && total < F(1e-30f)) return false;  // scores that fp32 cannot hold
+    score /= total == F(0) ? F(1) : total;
+  }
+  if (chosen) {
+    p.weights[row * p.top_k + lane] = float(score * F(p.scale));
+    p.ids[row * p.top_k + lane] = id;
+  }
+  return true;
+}
+
+template <typename T, int PER>
+__device__ __noinline__ void route_row_64(const RouteParams& p, int64_t row, int lane, const float* s_bias, double* s_keys) {
+  float x[PER];
+  load_logits<T, PER>(p, row, lane, x);
+  route_row<double, T, PER>(p, x, row, lane, s_bias, s_keys);
+}
+
+constexpr int kPutOff = 8;  // rows a warp puts off before it goes through them in 64 bits
+
+// Warps take rows in turn and load the next row's logits before they work on this one's.
+template <typename T, int PER, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 24 / WARPS) moe_route_kernel(const __grid_constant__ RouteParams p) {
+  __shared__ double s_keys[WARPS][32 * PER];  // (the fp32 rows use half)
+  __shared__ float4 s_bias4[PER * 8];
+  __shared__ int64_t s_put_off[WARPS][kPutOff];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* s_bias = reinterpret_cast<float*>(s_bias4);
+  if (p.bias) {
+    for (int e = threadIdx.x; e < 32 * PER; e += WARPS * 32) s_bias[e] = e < p.E ? __ldg(p.bias + e) : 0.f;
+    __syncthreads();
+  }
+  const int64_t step = int64_t(gridDim.x) * WARPS;
+  int64_t row = int64_t(blockIdx.x) * WARPS + warp;
+  while (row < p.M) {
+    int put_off = 0;
+    float x[PER];
+    load_logits<T, PER>(p, row, lane, x);
+    while (true) {
+      const int64_t next = row + step;
+      float ahead[PER];
+      if (next < p.M) load_logits<T, PER>(p, next, lane, ahead);
+      if (!route_row<float, T, PER>(p, x, row, lane, s_bias, reinterpret_cast<float*>(s_keys[warp]))) s_put_off[warp][put_off++] = row;
+      row = next;
+      if (row >= p.M || put_off == kPutOff) break;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) x[j] = ahead[j];
+    }
+    __syncwarp();
+    for (int i = 0; i < put_off; ++i) route_row_64<T, PER>(p, s_put_off[warp][i], lane, s_bias, s_keys[warp]);
+    __syncwarp();
+  }
+}
+
+// The usual shapes: top_k <= 8.  W lanes per token (several tokens per warp), lane s of them with experts s * PER .. s * PER + PER - 1 in
+// registers.  What the one-warp kernel spends on its rounds (37 instructions each) goes into networks of minima and maxima that
+// need no expert numbers: a lane sorts its keys eight at a time and merges them into its eight largest, a butterfly merges the lanes',
+// and the top_k-th of the result is all that is kept.  The keys that are not below it, less the tolerance, are the candidates,
+// top_k of them and rarely more; in a list, in expert order, each counts those before it, and that is its place.
+// 16384 tokens x 256 experts in groups, fp32 logits: one warp per token 980 instructions a row and 28 us, this kernel 430 and 17 us.
+// Where fp32 does not decide, the two comparisons that can be in doubt (between groups, between candidates) are made in 64
+// bits here, in little code: the whole row in 64 bits costs a launch 8 us, most of it fetching instructions that no other row has run.
+// A row with more candidates than the list holds, or too few keys above -infinity, goes to the general form.
+template <typename F, int N> __device__ __forceinline__ void merge_largest(F (&a)[N], const F (&b)[N]) {  // both sorted; a becomes the N largest
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = larger(a[i], b[N - 1 - i]);  // (a bitonic sequence)
+  merge_bitonic<N / 2>(a);
+}
+
+constexpr int kListCap = 16;
+
+template <typename T, int PER, int W, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel(const __grid_constant__ RouteParams p) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kRows = 32 / W;  // tokens a warp works on
+  __shared__ double s_keys[WARPS][W * PER <= 256 ? 256 : W * PER];  // for the rows that were put off (one warp per row: 32 lanes)
+  __shared__ float4 s_bias4[W * PER / 4];
+  __shared__ alignas(16) float s_key[WARPS][kRows][kListCap];
+  __shared__ float s_x[WARPS][kRows][kListCap];
+  __shared__ int s_id[WARPS][kRows][kListCap];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % W, mine = lane / W;
+  float* s_bias = reinterpret_cast<float*>(s_bias4);
+  if (p.bias) {
+    for (int e = threadIdx.x; e < W * PER; e += WARPS * 32) s_bias[e] = e < p.E ? __ldg(p.bias + e) : 0.f;
+    __syncthreads();
+  }
+  const float inf = __int_as_float(0x7f800000);
+  const int64_t row = (int64_t(blockIdx.x) * WARPS + warp) * kRows + mine;
+  const bool live = row < p.M;
+  const int e0 = sub * PER;
+  const bool by_logit = p.bias == nullptr && !p.summed;
+  const int present = min(max(p.E - e0, 0), PER);
+
+  float key[PER];
+  const T* src = reinterpret_cast<const T*>(p.logits) + (live ? row : 0) * p.ldl;
+  {
+    const bool on = present > 0;
+    if (p.wide) {
+#pragma unroll
+      for (int w = 0; w < PER; w += 4) {
+        float v[4];
+        load_word(src + e0 + w, on, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) key[w + j] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = j < present ? to_f32(src[e0 + j]) : 0.f;
+    }
+  }
+  auto across_max = [&](float v) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+    return v;
+  };
+  auto across_sum = [&](float v) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) v += __shfl_xor_sync(kAll, v, o);
+    return v;
+  };
+  // logits -> keys, the same arithmetic as route_row<float>
+  float top = 0.f, share = 1.f;
+  auto key_of = [&](float x, int e) {
+    if (by_logit) return x;
+    float k = p.softmax ? key_exp(x - top) * share : reciprocal(1.f + key_exp(-x));
+    if (p.bias) k += s_bias[e];
+    return k;
+  };
+  if (p.softmax) {
+    top = -inf;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) top = fmaxf(top, j < present ? key[j] : -inf);
+    top = across_max(top);
+    if (top == inf || top == -inf) top = 0.f;
+    float total = 0.f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) total += j < present ? key_exp(key[j] - top) : 0.f;
+    total = across_sum(total);
+    share = total == 0.f ? 1.f : reciprocal(total);
+  }
+  if (!by_logit) {
+    if (p.softmax) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = key_exp(key[j] - top) * share;
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = reciprocal(1.f + key_exp(-key[j]));
+    }
+    if (p.bias) {
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(s_bias + e0 + j);
+        key[j] += b.x; key[j + 1] += b.y; key[j + 2] += b.z; key[j + 3] += b.w;
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < PER; ++j) key[j] = e0 + j < p.E ? fmaxf(key[j], -inf) : nan;  // (a NaN key ranks with -infinity)
-  // How far a key can be off: `off` plus `rel` of its size.  The hardware exponential adds as much to the softmax as the
-  // argument's rounding does (route_row): 260 * 2^-24 of a score, which is at most `share`, the best one's.  A sigmoid p of x is off
-  // by p (1 - p) (|x| + 4) + 4 p roundings of 2^-24, at most 5.4 of them.
-  const float off = by_logit ? 0.f : (p.softmax ? 1.6e-5f * share : 1e-6f) + 1e-37f;
-  const float rel = by_logit ? 0.f : 2.4e-7f;
-  bool sure = true;
+  for (int j = 0; j < PER; ++j) key[j] = fmaxf(key[j], -inf);  // (a NaN key ranks with -infinity)
+  if (present < PER) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = j < present ? key[j] : -inf;
+  }
+  const bool check = !by_logit;
+  const float off = check ? (p.softmax ? 1.6e-5f * share : 3.4e-7f) + 1e-37f : 0.f;  // how far a key can be off, see route_row
+  const float rel = check ? 1.2e-7f : 0.f;
+  bool in = present > 0;
+  // the same in 64 bits, where fp32 does not decide
+  double total_64 = 0.0;
+  auto need_total_64 = [&]() {
+    if (!p.softmax || total_64 != 0.0) return;
+#pragma unroll 2
+    for (int j = 0; j < PER; ++j) total_64 += j < present ? exp(double(to_f32(src[e0 + j])) - double(top)) : 0.0;
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) total_64 += __shfl_xor_sync(kAll, total_64, o);
+    if (total_64 == 0.0) total_64 = 1.0;
+  };
+  auto score_64 = [&](float v) {
+    const double z = exp(p.softmax ? double(v) - double(top) : -double(v));
+    return p.softmax ? z / total_64 : 1.0 / (1.0 + z);
+  };
 
-  bool in = e0 < p.E;
   if (p.groups > 1) {
-    const int lanes = p.group_size / PER, g = lane / lanes;  // (whole groups of lanes, checked on the host)
-    float a = -inf, b = -inf;  // the group's two largest keys
+    // (groups are whole lanes, a power of two of them: checked on the host)
+    const int lanes = p.group_size / PER, g = sub / lanes;
+    const bool two = p.summed && p.group_size > 1;
+    float a = -inf, b = -inf;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       b = fmaxf(b, fminf(a, key[j]));
       a = fmaxf(a, key[j]);
     }
     for (int o = 1; o < lanes; o <<= 1) {
-      const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+      const float a2 = __shfl_xor_sync(kAll, a, o), b2 = __shfl_xor_sync(kAll, b, o);
       b = fmaxf(fminf(a, a2), fmaxf(b, b2));
       a = fmaxf(a, a2);
     }
-    const bool two = p.summed && p.group_size > 1;
     const float value = two ? fmaxf(a + b, -inf) : a;
-    int rank = 0;
-    for (int h = 0; h < p.groups; ++h) {
-      const float other = __shfl_sync(0xffffffffu, value, h * lanes);
-      rank += (other > value || (other == value && h < g)) ? 1 : 0;
-    }
-    const bool chosen = rank < p.topk_groups;
-    if (!by_logit && p.topk_groups < p.groups) {
+    auto rank_of = [&](auto v) {
+      int rank = 0;
+#pragma unroll 4
+      for (int h = 0; h < p.groups; ++h) {
+        const auto other = __shfl_sync(kAll, v, mine * W + h * lanes);
+        rank += (other > v || (other == v && h < g)) ? 1 : 0;
+      }
+      return rank;
+    };
+    bool chosen = rank_of(value) < p.topk_groups;
+    if (check && p.topk_groups < p.groups) {
       const float slack = 2.f * off + rel * (fabsf(a) + (two ? fabsf(b) : 0.f) + fabsf(value));
-      const float worst_in = -warp_max_f32(in && chosen ? slack - value : -inf);  // what the worst in and the best out can be
-      const float best_out = warp_max_f32(in && !chosen ? value + slack : -inf);
-      if (!(worst_in > best_out)) sure = false;
+      const float worst_in = -across_max(in && chosen ? slack - value : -inf);  // what the worst in and the best out can be
+      const float best_out = across_max(in && !chosen ? value + slack : -inf);
+      if (__any_sync(kAll, live && !(worst_in > best_out))) {
+        need_total_64();
+        const float near = (two ? b : a) - 2.1f * (off + rel * fabsf(two ? b : a));  // keys that can be among the group's two largest
+        uint32_t maybe = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) maybe |= (j < present && !(key[j] < near)) ? 1u << j : 0u;
+        double a64 = -double(inf), b64 = -double(inf);
+        for (; __any_sync(kAll, maybe != 0); maybe &= maybe - 1u) {
+          if (maybe != 0) {
+            const int e = e0 + __ffs(maybe) - 1;
+            double v = score_64(to_f32(src[e]));
+            if (p.bias) v += double(s_bias[e]);
+            if (v > a64) { b64 = a64; a64 = v; }
+            else if (v > b64) b64 = v;
+          }
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+          const double a2 = __shfl_xor_sync(kAll, a64, o), b2 = __shfl_xor_sync(kAll, b64, o);
+          const double lesser = a2 > a64 ? a64 : a2;
+          b64 = b2 > b64 ? b2 : b64;
+          b64 = lesser > b64 ? lesser : b64;
+          a64 = a2 > a64 ? a2 : a64;
+        }
+        chosen = rank_of(two ? larger(a64 + b64, -double(inf)) : a64) < p.topk_groups;
+      }
     }
     in = in && chosen;
   }
 
-  // a bound from below on the top_k-th largest key
-  float lane_top = nan;
-  if (in) {
+  // the top_k-th largest key
+  float best[8];
+  if constexpr (PER >= 8) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) lane_top = fmaxf(lane_top, key[j]);
+    for (int j = 0; j < 8; ++j) best[j] = key[j];
+    sort_descending(best);
+#pragma unroll
+    for (int c = 8; c < PER; c += 8) {
+      float more[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) more[j] = key[c + j];
+      sort_descending(more);
+      merge_largest(best, more);
+    }
   }
-  float floor_key = -inf;
-  for (int i = 0; i < p.top_k; ++i) {
-    const float m = warp_max_f32(lane_top);
-    floor_key = m;
-    if (m != m) break;  // fewer lanes than choices: every key that is there
-    const uint32_t at = __ballot_sync(0xffffffffu, lane_top == m);
-    if (lane == __ffs(at) - 1) lane_top = nan;
+  if (!in) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) best[j] = -inf;
   }
-  if (!by_logit) floor_key -= 2.1f * (off + rel * fabsf(floor_key));
-  if (floor_key != floor_key) floor_key = -inf;  // (also -infinity less its own size)
-  // the keys that are not below it, one per lane
+#pragma unroll
+  for (int o = 1; o < W; o <<= 1) {
+    float other[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) other[j] = __shfl_xor_sync(kAll, best[j], o);
+    merge_largest(best, other);
+  }
+  float least = best[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) least = j < p.top_k ? best[j] : least;
+  if (check) least -= 2.1f * (off + rel * fabsf(least));
+  bool odd = !(least > -inf);  // fewer keys than choices above -infinity: the general form knows what is there
+
+  // candidates, in expert order
   uint32_t picked = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) picked |= (in && key[j] >= floor_key) ? 1u << j : 0u;
-  const int mine = __popc(picked);
-  int upto = mine;
+  for (int j = 0; j < PER; ++j) picked |= key[j] >= least ? 1u << j : 0u;
+  if (!in || !live) picked = 0;
+  int upto = __popc(picked);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += t;
+  for (int o = 1; o < W; o <<= 1) {
+    const int t = __shfl_up_sync(kAll, upto, o);
+    if (sub >= o) upto += t;
   }
-  const int count = __shfl_sync(0xffffffffu, upto, 31);
-  if (count > 32) return route_slowly<T, PER>(p, row, lane, true);
-  int at = upto - mine;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    if ((picked >> j) & 1u) {
-      s_key[warp][at] = make_float2(key[j], x[j]);
-      s_id[warp][at] = e0 + j;
+  const int count = __shfl_sync(kAll, upto, mine * W + W - 1);
+  int at = upto - __popc(picked);
+  if (count > kListCap) odd = true;
+  if (odd) picked = 0;
+  while (__any_sync(kAll, picked != 0)) {
+    if (picked != 0) {
+      const int j = __ffs(picked) - 1;
+      picked &= picked - 1u;
+      const float x = to_f32(src[e0 + j]);
+      s_key[warp][mine][at] = fmaxf(key_of(x, e0 + j), -inf);
+      s_x[warp][mine][at] = x;
+      s_id[warp][mine][at] = e0 + j;
       ++at;
     }
   }
   __syncwarp();
-  const float2 kx = lane < count ? s_key[warp][lane] : make_float2(0.f, 0.f);
-  const int id = lane < count ? s_id[warp][lane] : 0;
-  const float k = kx.x;
-  int rank = 0;  // list order is expert order: equal keys keep it
-  for (int t = 0; t < count; ++t) {
-    const float other = __shfl_sync(0xffffffffu, k, t);
-    rank += (other > k || (other == k && t < lane)) ? 1 : 0;
+  // every lane counts those before its candidates sub and sub + 8; then lane s holds choice s
+  const int listed = odd ? 0 : count;
+  float cx[2], ck[2];
+  int place[2], cid[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int t = sub + 8 * c;
+    const bool on = sub < 8 && t < listed;
+    ck[c] = on ? s_key[warp][mine][t] : 0.f;
+    cx[c] = on ? s_x[warp][mine][t] : 0.f;
+    cid[c] = on ? s_id[warp][mine][t] : 0;
+    place[c] = on ? 0 : kListCap;
   }
-  __syncwarp();
-  if (lane < count) {
-    s_key[warp][rank] = kx;
-    s_id[warp][rank] = id;
+  const bool more = __any_sync(kAll, listed > 8);
+#pragma unroll 2
+  for (int t = 0; t < (more ? kListCap : 8); ++t) {
+    const float other = t < listed ? s_key[warp][mine][t] : -inf;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) place[c] += (other > ck[c] || (other == ck[c] && t < sub + 8 * c && t < listed)) ? 1 : 0;
   }
-  __syncwarp();
-  const bool chosen = lane < p.top_k;
-  const int best = chosen ? s_id[warp][lane] : 0;
-  const float2 bx = chosen ? s_key[warp][lane] : make_float2(0.f, 0.f);
-  if (!by_logit && chosen && lane + 1 < count) {
-    const float next = s_key[warp][lane + 1].x;
-    if (!(bx.x - next > 2.f * off + rel * (fabsf(bx.x) + fabsf(next)))) sure = false;
+  bool chosen = false;
+  float k = 0.f, x = 0.f;
+  auto in_order = [&]() {
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (place[c] < kListCap) {
+        s_key[warp][mine][place[c]] = ck[c];
+        s_x[warp][mine][place[c]] = cx[c];
+        s_id[warp][mine][place[c]] = cid[c];
+      }
+    }
+    __syncwarp();
+    chosen = sub < p.top_k && sub < listed;
+    k = chosen ? s_key[warp][mine][sub] : 0.f;
+    x = chosen ? s_x[warp][mine][sub] : 0.f;
+  };
+  in_order();
+  if (check) {
+    const float next = chosen && sub + 1 < listed ? s_key[warp][mine][sub + 1] : -inf;
+    if (__any_sync(kAll, live && chosen && sub + 1 < listed && !(k - next > 2.f * off + rel * (fabsf(k) + fabsf(next))))) {
+      need_total_64();
+      double k64[2];
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        const double v = score_64(c == 0 ? cx[0] : cx[1]) + (p.bias ? double(s_bias[c == 0 ? cid[0] : cid[1]]) : 0.0);
+        if (c == 0) k64[0] = larger(v, -double(inf));
+        else k64[1] = larger(v, -double(inf));
+        if (!more) break;
+      }
+      if (!more) k64[1] = 0.0;
+      place[0] = sub < 8 && sub < listed ? 0 : kListCap;
+      place[1] = sub < 8 && sub + 8 < listed ? 0 : kListCap;
+#pragma unroll 1
+      for (int t = 0; t < kListCap; ++t) {
+        const double other = __shfl_sync(kAll, t < 8 ? k64[0] : k64[1], mine * W + (t & 7));
+        if (t < listed) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) place[c] += (other > k64[c] || (other == k64[c] && t < sub + 8 * c)) ? 1 : 0;
+        }
+      }
+      in_order();
+    }
   }
-  // the scores of the chosen alone, with the exponential that is right to two units in the last place
-  float sc = p.softmax ? expf(bx.y - top) * share : __fdividef(1.f, 1.f + expf(-bx.y));
+  float score = 0.f;
+  if (chosen) score = p.softmax ? expf(x - top) * share : __fdividef(1.f, 1.f + expf(-x));
   if (p.renormalize) {
-    float total = warp_sum(chosen ? sc : 0.f);
-    if (total < 1e-30f) sure = false;  // scores that fp32 cannot hold
-    sc = __fdiv_rn(sc, total);
+    const float total = across_sum(score);
+    if (__any_sync(kAll, live && !odd && total < 1e-30f)) {  // scores that fp32 cannot hold
+      need_total_64();
+      const double exact = chosen ? score_64(x) : 0.0;
+      double sum = exact;
+#pragma unroll
+      for (int o = 1; o < W; o <<= 1) sum += __shfl_xor_sync(kAll, sum, o);
+      score = float(exact / (sum == 0.0 ? 1.0 : sum));
+    } else {
+      score = __fdividef(score, total);
+    }
   }
-  if (!__all_sync(0xffffffffu, sure)) return route_slowly<T, PER>(p, row, lane, false);
-  write_choice(p, row, lane, best, sc * p.scale);
+  if (chosen && live) {
+    p.weights[row * p.top_k + sub] = score * p.scale;
+    p.ids[row * p.top_k + sub] = s_id[warp][mine][sub];
+  }
+  const uint32_t again = __ballot_sync(kAll, odd && live);
+#pragma unroll 1
+  for (int r = 0; r < kRows; ++r) {
+    if ((again >> (r * W)) & 1u) {
+      __syncwarp();
+      route_row_64<T, (W * PER + 31) / 32>(p, (int64_t(blockIdx.x) * WARPS + warp) * kRows + r, lane, s_bias, s_keys[warp]);
+    }
+  }
+}
+
+template <typename T, int PER, int W>
+int launch_route_lists(RouteParams p, cudaStream_t st) {
+  constexpr int kWarps = 4, kPer64 = (W * PER + 31) / 32;
+  const int64_t rows = kWarps * (32 / W);
+  p.wide = p.E % PER == 0 && reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && (p.ldl * int64_t(sizeof(T))) % 16 == 0;
+  const int lanes = p.group_size / kPer64;  // (of the 64-bit form)
+  p.whole_lanes = p.group_size % kPer64 == 0 && (lanes & (lanes - 1)) == 0;
+  moe_route_lists_kernel<T, PER, W, kWarps><<<unsigned((p.M + rows - 1) / rows), kWarps * 32, 0, st>>>(p);
+  return check_cuda(cudaGetLastError(), "moe_route launch");
+}
+// whether a group is a power of two of lanes with PER experts each
+inline bool whole_lanes(const RouteParams& p, int per) {
+  const int lanes = p.group_size / per;
+  return p.groups == 1 || (p.group_size % per == 0 && (lanes & (lanes - 1)) == 0);
 }
 
 template <typename T, int PER>
 int launch_route_per(RouteParams p, cudaStream_t st) {
-  const unsigned grid = unsigned((int64_t(p.M) + kRouteWarps - 1) / kRouteWarps);
+  constexpr int kWarps = PER >= 32 ? 4 : 8;
   // lanes read whole words where every row starts on one and a lane has all of its experts or none
+  const bool full = p.E % PER == 0;
   const int word = PER * int(sizeof(T)) < 16 ? PER * int(sizeof(T)) : 16;
-  p.wide = p.E % PER == 0 && reinterpret_cast<uintptr_t>(p.logits) % word == 0 && (p.ldl * int64_t(sizeof(T))) % word == 0;
-  p.wide_bias = p.E % PER == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+  p.wide = full && reinterpret_cast<uintptr_t>(p.logits) % word == 0 && (p.ldl * int64_t(sizeof(T))) % word == 0;
   const int lanes = p.group_size / PER;
-  p.slow_groups = p.groups > 1 && (p.group_size % PER != 0 || (lanes & (lanes - 1)) != 0);
-  moe_route_kernel<T, PER><<<grid, kRouteWarps * 32, 0, st>>>(p);
+  p.whole_lanes = p.group_size % PER == 0 && (lanes & (lanes - 1)) == 0;
+  const int64_t blocks = (int64_t(p.M) + kWarps - 1) / kWarps, resident = int64_t(sm_count()) * (24 / kWarps);
+  moe_route_kernel<T, PER, kWarps><<<unsigned(blocks < resident ? blocks : resident), kWarps * 32, 0, st>>>(p);
   return check_cuda(cudaGetLastError(), "moe_route launch");
 }
 
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t st) {
+  if (p.top_k <= 8 && p.E > 32) {
+    if (p.E <= 64 && whole_lanes(p, 8)) return launch_route_lists<T, 8, 8>(p, st);
+    if (p.E > 64 && p.E <= 128 && whole_lanes(p, 16)) return launch_route_lists<T, 16, 8>(p, st);
+    if (p.E > 128 && p.E <= 256 && whole_lanes(p, 32)) return launch_route_lists<T, 32, 8>(p, st);
+    if (p.E > 256 && p.E <= 512 && whole_lanes(p, 32)) return launch_route_lists<T, 32, 16>(p, st);
+  }
   const int per = (p.E + 31) / 32;
   if (per <= 1) return launch_route_per<T, 1>(p, st);
   if (per <= 2) return launch_route_per<T, 2>(p, st);

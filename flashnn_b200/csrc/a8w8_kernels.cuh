@@ -196,16 +196,30 @@ __device__ __forceinline__ void store_chunk_moe(const uint32_t (&r)[32], int64_t
 template <int BN, class FX>
 __device__ __forceinline__ void stage_columns(float* cs, int j0, int count, int n0, int64_t col_base, int lane, const A8W8Params& p,
                                               const FX& fx) {
-  for (int j = j0 + lane; j < j0 + count; j += 32) {
-    if constexpr (FX::kOn) {
-      constexpr int OW = FX::kGated ? BN / 2 : BN;
-      const int n = n0 + (j < OW ? j : j - OW);
-      const int64_t at = col_base + n + (j < OW ? 0 : p.N);
-      cs[j] = n < p.N ? load_as_f32(p.alpha_col, p.col_dtype, at) : 0.f;
-      cs[BN + j] = (n < p.N && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, at) : 0.f;
-    } else {
-      cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
+  if constexpr (FX::kOn) {
+    // four columns of a lane at a time: their loads are in flight together
+    constexpr int OW = FX::kGated ? BN / 2 : BN;
+    for (int j = j0 + lane; j < j0 + count; j += 128) {
+      float s[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = j + 32 * i, n = n0 + (c < OW ? c : c - OW);
+        const int64_t at = col_base + n + (c < OW ? 0 : p.N);
+        const bool on = c < j0 + count && n < p.N;
+        s[i] = on ? load_as_f32(p.alpha_col, p.col_dtype, at) : 0.f;
+        b[i] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, at) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (j + 32 * i < j0 + count) {
+          cs[j + 32 * i] = s[i];
+          cs[BN + j + 32 * i] = b[i];
+        }
+      }
     }
+  } else {
+    for (int j = j0 + lane; j < j0 + count; j += 32)
+      cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
   }
 }
 
@@ -216,12 +230,12 @@ template <int BN, class FX>
 __device__ __forceinline__ void fused_chunk(const uint32_t (&r)[32], const uint32_t (&u)[32], float rs, const float* cs, int c32,
                                             bool same16, const A8W8Params& p, const FX& fx, float (&v)[32]) {
   scale_chunk(r, rs, cs + c32, same16, p, v);
-  add_bias32(cs + BN + c32, v);
+  if (fx.bias) add_bias32(cs + BN + c32, v);
   activate_n(v, fx.act);
   if constexpr (FX::kGated) {
     float w[32];
     scale_chunk(u, rs, cs + BN / 2 + c32, same16, p, w);
-    add_bias32(cs + BN + BN / 2 + c32, w);
+    if (fx.bias) add_bias32(cs + BN + BN / 2 + c32, w);
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] *= w[j];
   }
@@ -788,15 +802,28 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     const bool same16 = !MOE && (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
     const bool vec_ok = (p.ldo % 8 == 0) && (reinterpret_cast<uintptr_t>(p.out) % 16 == 0);
     const bool acc_vec_ok = p.acc_out && (p.ldacc % 4 == 0) && (reinterpret_cast<uintptr_t>(p.acc_out) % 16 == 0);
+    const int my_row = int(rank) * 128 + quarter * 32 + lane;           // this thread's row within a tile
     bool res_vec_ok = false;
     if constexpr (FX::kOn) res_vec_ok = (fx.ldr % 8 == 0) && (reinterpret_cast<uintptr_t>(fx.residual) % 16 == 0);
+    auto load_res = [&](int row, int col0, uint32_t (&r)[16]) { load_residual32<OutT>(fx, row, col0, p.M, p.N, res_vec_ok, r); };
+    // this thread's piece of the next tile's residual -> L2, a tile ahead
+    auto prefetch_res = [&](PairWork<SK, MOE> ahead) {
+      if constexpr (FX::kOn) {
+        if (!ahead.next()) return;
+        int mb, nb;
+        tile_coords(ahead.tile, p.tiles_m, p.tiles_n, mb, nb);
+        const int row = mb * 256 + my_row, col0 = nb * OW + c_begin * 32, col1 = min(nb * OW + c_end * 32, p.N);
+        if (row >= p.M) return;
+        const OutT* src = reinterpret_cast<const OutT*>(fx.residual) + int64_t(row) * fx.ldr;
+        for (int c = col0; c < col1; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
+      }
+    };
     int local = 0;
     bool ok = true;
     PairWork<SK, MOE> w(p, pair_id, num_pairs);
     uint8_t* out_stage = smem + L::kOutOff + ewarp * (L::kOutBufs * 2048);  // this warp's output staging buffer(s)
     int out_buf = 0;
     const int my_flag = int(rank) * 4 + quarter;                        // this warp's flag word within a pair's eight
-    const int my_row = int(rank) * 128 + quarter * 32 + lane;           // this thread's row within a tile
     for (; ok && w.next(); ++local) {
       int mb, nb;
       tile_coords(w.tile, p.tiles_m, p.tiles_n, mb, nb);
@@ -833,6 +860,13 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         }
       } else {
         rs = (row < p.M) ? load_as_f32(p.alpha_row, p.row_dtype, row) : 0.f;
+      }
+      uint32_t res[16];
+      if constexpr (FX::kOn) {
+        if (!MOE && fx.residual) {
+          load_res(row, n0 + c_begin * 32, res);
+          prefetch_res(w);
+        }
       }
       __syncwarp();
 
@@ -873,9 +907,9 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         uint32_t r[32], u[32];
         tmem_ld_32x32(taddr + c * 32, r);
         if (FX::kGated) tmem_ld_32x32(taddr + OW + c * 32, u);
-        uint32_t res[16];
+        uint32_t res_next[16];  // the residual is loaded a chunk ahead
         if constexpr (FX::kOn) {
-          if (!MOE && fx.residual) load_residual32<OutT>(fx, row, n0 + c * 32, p.M, p.N, res_vec_ok, res);
+          if (!MOE && fx.residual && c + 1 < c_end) load_res(row, n0 + (c + 1) * 32, res_next);
         }
         uint4 cur[8];
         if (adds) {
@@ -912,7 +946,11 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         float v[32];
         if constexpr (FX::kOn) {
           fused_chunk<BN>(r, u, rs, cs, c * 32, same16, p, fx, v);
-          if (!MOE && fx.residual) add_residual32<OutT>(res, v);
+          if (!MOE && fx.residual) {
+            add_residual32<OutT>(res, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) res[j] = res_next[j];
+          }
         }
         if (MOE && FX::kOn) {
           if (out_row >= 0 && n0 + c * 32 < p.N) store_values<OutT>(v, out_row, n0 + c * 32, p, vec_ok);

@@ -28,15 +28,36 @@ template <bool GATED> struct FusedEpilogue {
   int experts;           // fused MoE: slots of a block whose expert is not one of these write nothing
 };
 
-// 1 / (1 + e^-v) by the hardware's exponential and reciprocal: a few 2^-22 off, far below the half step (2^-9, 2^-12) of
-// the 16-bit output.  e^-v of a very negative v is infinite and its reciprocal 0; a NaN stays one.
-__device__ __forceinline__ float sigmoid_f32(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// The hardware's 2^v and reciprocal as they are (subnormal results flushed to 0): one instruction each, where __expf and
+// __fdividef add the scaling that keeps subnormals.  With K short the epilogue is what a tile waits for, and these are its longest part.
+__device__ __forceinline__ float exp2_ftz(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_ftz(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / (1 + e^-v): within (|v| + 8) roundings of 2^-24, far below the half step (2^-9, 2^-12) of the 16-bit output.  e^-v of a
+// very negative v is infinite and its reciprocal 0 (from v = -87.3 on); a NaN stays one.
+__device__ __forceinline__ float sigmoid_f32(float v) { return rcp_ftz(1.f + exp2_ftz(-1.4426950408889634f * v)); }
+// v Phi(v), Phi(v) = erfc(-v / sqrt 2) / 2, with erfc(x) = (a1 t + ... + a5 t^5) e^(-x^2), t = 1 / (1 + 0.3275911 x) for x >= 0
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26): within 1.5e-7, where erff takes three times the instructions.
+__device__ __forceinline__ float gelu_f32(float v) {
+  const float x = fabsf(v) * 0.70710678118654752f;
+  const float t = rcp_ftz(fmaf(0.3275911f, x, 1.f));
+  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  const float tail = 0.5f * poly * exp2_ftz(-1.4426950408889634f * (x * x));
+  return v * (v > 0.f ? 1.f - tail : tail);
+}
 
 template <int ACT> __device__ __forceinline__ float activate(float v) {
   if (ACT == FNN_ACT_RELU) return v < 0.f ? 0.f : v;  // (keeps a NaN)
   if (ACT == FNN_ACT_SIGMOID) return sigmoid_f32(v);
   if (ACT == FNN_ACT_SILU) return v * sigmoid_f32(v);
-  if (ACT == FNN_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  if (ACT == FNN_ACT_GELU) return gelu_f32(v);
   // v / 2 (1 + tanh(t)) = v sigmoid(2 t)
   if (ACT == FNN_ACT_GELU_TANH) return v * sigmoid_f32(1.5957691216057308f * fmaf(0.044715f * v, v * v, v));
   return v;

@@ -7,7 +7,7 @@ import torch
 from . import _lib
 from .fused_moe import _i32
 from .kernel_backend import BackendKernel
-from .quant_gemm import _DT, _on_device, _require_cuda, _stream
+from .quant_gemm import _DT, _flat, _on_device, _one_device, _stream
 
 
 class MoeRouting(BackendKernel):
@@ -33,7 +33,7 @@ class MoeRouting(BackendKernel):
         self.num_groups, self.topk_groups, self.group_score = num_groups, topk_groups, group_score
 
     def _cuda_impl(self, logits, bias=None):
-        _require_cuda(logits, bias)
+        _one_device(logits, bias)
         assert logits.dim() == 2 and logits.shape[1] == self.num_experts, "logits must be [M, num_experts]"
         assert logits.dtype in _DT, "logits must be float16, bfloat16 or float32"
         m, e = logits.shape
@@ -41,7 +41,7 @@ class MoeRouting(BackendKernel):
             logits = logits.contiguous()
         if bias is not None:
             assert bias.numel() == e and bias.is_floating_point(), "bias must be [num_experts]"
-            bias = bias.reshape(-1).to(torch.float32).contiguous()
+            bias = _flat(bias if bias.dtype == torch.float32 else bias.float())
         weights = logits.new_empty((m, self.top_k), dtype=torch.float32)
         ids = logits.new_empty((m, self.top_k), dtype=torch.int32)
         with _on_device(logits):
@@ -63,7 +63,7 @@ def moe_sort_tokens(topk_ids, num_experts, BM, first_expert=0):
     Experts are first_expert .. first_expert + num_experts - 1 and numbered from 0 in expert_ids; a choice of any other
     expert (one of another device, or -1) gets no slot.  EM depends on the sizes alone: the most slots that any choice of
     experts fills."""
-    _require_cuda(topk_ids)
+    _one_device(topk_ids)
     assert topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64"
     assert num_experts >= 1 and BM >= 1, "num_experts and BM must be positive"
     ids = _i32(topk_ids).contiguous()
@@ -83,14 +83,16 @@ def moe_combine(C, topk_weights=None, topk_ids=None, num_experts=None, first_exp
 
     With topk_ids [M, top_k] choices of experts outside first_expert .. first_expert + num_experts - 1 are left out: the
     expert products did not write their rows of C, which are not read."""
-    _require_cuda(C, topk_weights, topk_ids, residual)
+    _one_device(C, topk_weights, topk_ids, residual)
     assert C.dim() == 3 and C.dtype in (torch.float16, torch.bfloat16), "C must be [M, top_k, N] in float16 or bfloat16"
     m, k, n = C.shape
     if n > 1 and C.stride(2) != 1:
         C = C.contiguous()
     if topk_weights is not None:
         assert topk_weights.shape == (m, k) and topk_weights.dtype in _DT, "topk_weights must be [M, top_k] in a float dtype"
-        topk_weights = topk_weights.float().contiguous()
+        topk_weights = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
+        if not topk_weights.is_contiguous():
+            topk_weights = topk_weights.contiguous()
     if topk_ids is not None:
         assert topk_ids.shape == (m, k) and num_experts is not None and num_experts >= 1, "topk_ids must be [M, top_k], with num_experts"
         topk_ids = _i32(topk_ids).contiguous()

@@ -45,7 +45,7 @@ class _on_device:
         self.ctx = None
 
     def __enter__(self):
-        if torch.cuda.current_device() != self.index:
+        if torch._C._cuda_getDevice() != self.index:
             self.ctx = torch.cuda.device(self.index)
             self.ctx.__enter__()
 
@@ -61,6 +61,20 @@ def _require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("flashnn_b200 operators need CUDA tensors; there is no CPU path")
+
+
+def _one_device(first, *others):
+    """Refuses CPU tensors and tensors of different devices (None is left out)."""
+    index = first.get_device()
+    for t in (first, *others):
+        if t is not None and t.get_device() != index or index < 0:
+            _require_cuda(first, *others)
+            raise RuntimeError("flashnn_b200 operators need all tensors on one device")
+
+
+def _flat(t):
+    """t as a contiguous vector; free for one (a reshape costs a microsecond)."""
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
 
 class DynamicQuantize(BackendKernel):
@@ -155,7 +169,7 @@ class GemmA8W8Epilogue(BackendKernel):
         self.gated = bool(gated)
 
     def _cuda_impl(self, a, b, alpha_row, alpha_col, bias=None, residual=None):
-        _require_cuda(a, b, alpha_row, alpha_col, bias, residual)
+        _one_device(a, b, alpha_row, alpha_col, bias, residual)
         assert a.dim() == 2 and b.dim() == 2, "Matrix A/B must be 2-D"
         assert a.dtype == torch.int8 and b.dtype == torch.int8, "Matrix A/B must be int8 type"
         assert self.out_ty in (torch.float16, torch.bfloat16), "Output type must be float16 or bfloat16"
@@ -163,16 +177,16 @@ class GemmA8W8Epilogue(BackendKernel):
         (m, k), rows = a.shape, b.shape[0]
         assert not self.gated or rows % 2 == 0, "with a gate matrix B must have an even number of rows"
         n = rows // 2 if self.gated else rows
+        lda, ldb = (a.stride(0) if m > 1 else k), (b.stride(0) if rows > 1 else k)
         if k > 1 and a.stride(1) != 1:
-            a = a.contiguous()
+            a, lda = a.contiguous(), k
         if k > 1 and b.stride(1) != 1:
-            b = b.contiguous()
-        row = alpha_row.reshape(-1).contiguous()
-        col = alpha_col.reshape(-1).contiguous()
+            b, ldb = b.contiguous(), k
+        row, col = _flat(alpha_row), _flat(alpha_col)
         assert row.numel() == m and col.numel() == rows, "scale shapes must be [M] and [N] (2 N with a gate)"
         assert row.dtype in _DT and col.dtype in _DT, "scales must be float16, bfloat16 or float32"
         if bias is not None:
-            bias = bias.reshape(-1).contiguous()
+            bias = _flat(bias)
             assert bias.numel() == rows and bias.dtype in _DT, "bias must be [N] (2 N with a gate) in a float dtype"
         ldr = 0
         if residual is not None:
@@ -180,10 +194,10 @@ class GemmA8W8Epilogue(BackendKernel):
             if n > 1 and residual.stride(1) != 1:
                 residual = residual.contiguous()
             ldr = residual.stride(0) if m > 1 else n
-        out = torch.empty([m, n], dtype=self.out_ty, device=a.device)
+        out = a.new_empty((m, n), dtype=self.out_ty)
         with _on_device(a):
             _lib.check(_lib.lib().fnn_gemm_a8w8_epilogue(
-                a.data_ptr(), a.stride(0) if m > 1 else k, b.data_ptr(), b.stride(0) if rows > 1 else k,
+                a.data_ptr(), lda, b.data_ptr(), ldb,
                 row.data_ptr(), _DT[row.dtype], col.data_ptr(), _DT[col.dtype],
                 bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0,
                 _lib.ACTIVATIONS[self.activation], int(self.gated),

@@ -25,9 +25,10 @@ def activate(v, name):
 
 def activation_error(v, y, name):
     """How far an fp32 evaluation at v may be off y = activate(v): the hardware exponential is within 2 + 1.173 |x| steps of
-    2^-23, reciprocal, sum and products within 6 more; erf is within 2 steps of 2^-24 of at most 1 and 3 roundings follow."""
+    2^-23, reciprocal, sum and products within 6 more; where the sigmoid is below 2^-126 (|v| < 2^7) it may be taken as 0.
+    The erf is within 1.5e-7 < 2.6 * 2^-24, of which half goes into Phi, and 2.7 roundings of at most 1 follow."""
     if name in ("sigmoid", "silu"):
-        return y.abs() * 2 * U32 * (8 + 1.2 * v.abs())
+        return y.abs() * 2 * U32 * (8 + 1.2 * v.abs()) + 2.0 ** -119
     if name == "gelu":
         return v.abs() * 4 * U32
     if name == "gelu_tanh":

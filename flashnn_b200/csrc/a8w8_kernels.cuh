@@ -67,11 +67,34 @@ struct A8W8Params {
   int sk_tiles, sk_units, sk_tail_units, sk_slots;  // sk_slots: slots reserved per tail-sharing pair
 };
 
+constexpr int kMaxRuns = 1024;  // blocks of a slot list that can be gathered into runs
+
+// Runs of consecutive blocks of one expert, at most `most` blocks long: runs[i] becomes run i's first block, runs[count] the number
+// of blocks in use.  One warp; the list has at most kMaxRuns blocks.
+__device__ __forceinline__ int find_runs(const int32_t* expert_ids, int blocks, int most, int lane, int* runs) {
+  int count = 0, head = 0;  // head: first block of the current expert
+  for (int b0 = 0; b0 < blocks; b0 += 32) {
+    const int b = b0 + lane;
+    const bool on = b < blocks;
+    const int e = on ? __ldg(expert_ids + b) : 0;
+    const bool first = on && (b == 0 || __ldg(expert_ids + b - 1) != e);
+    const uint32_t heads = __ballot_sync(0xffffffffu, first) & (0xffffffffu >> (31 - lane));
+    const int from = heads ? b0 + 31 - __clz(heads) : head;
+    const bool start = on && (b - from) % most == 0;
+    const uint32_t starts = __ballot_sync(0xffffffffu, start);
+    if (start) runs[count + __popc(starts & ((1u << lane) - 1u))] = b;
+    count += __popc(starts);
+    head = __shfl_sync(0xffffffffu, from, 31);
+  }
+  if (lane == 0) runs[count] = blocks;
+  return count;
+}
+
 // AROWS: rows of A one stage holds (16, 32, 64 or 128).  Decode shapes are bound by the weight stream, and what
 // bounds that is the bytes a CTA keeps in flight, so their stages carry only the rows of A that exist and there are
 // more of them.  The tensor core still reads 128 rows from the A base (what lies behind the real rows belongs to the
 // following buffers; the accumulator rows it produces are never stored), so the last stage is followed by padding.
-template <int BN, int STAGES, int AROWS = kBM, bool BIAS = false> struct SmemLayout {
+template <int BN, int STAGES, int AROWS = kBM, bool BIAS = false, bool RUNS = false> struct SmemLayout {
   static constexpr int kColWords = (BIAS ? 2 : 1) * BN;  // per epilogue warp: column scales, then (fused epilogue) biases
   static constexpr int kABytes = AROWS * kBK;
   static constexpr int kBBytes = BN * kBK;
@@ -82,7 +105,8 @@ template <int BN, int STAGES, int AROWS = kBM, bool BIAS = false> struct SmemLay
   static constexpr int kNumBars = 2 * STAGES + 4 + 1;                // full, empty, tmem full/empty x2, drain
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kAbortOff = kTmemSlotOff + 8;
-  static constexpr int kTotal = kAbortOff + 8;
+  static constexpr int kRunsOff = kAbortOff + 8;       // [kMaxRuns + 2] first block of each run; the last word is their number
+  static constexpr int kTotal = kRunsOff + (RUNS ? 4 * (kMaxRuns + 2) : 0);
   static constexpr int kDynamicBytes = kTotal + 1024;  // slack for manual 1024-byte alignment
 };
 
@@ -260,11 +284,12 @@ __device__ __forceinline__ void store_values(const float (&v)[32], int64_t row, 
 
 // FX: NoEpilogue, or the fused epilogue (epilogue.cuh).  With a gate a tile has BN / 2 output columns: its BN accumulator
 // columns are BN / 2 weight rows of each half.
-template <typename OutT, int BN, int STAGES, bool MOE, int AROWS, class FX = NoEpilogue>
+template <typename OutT, int BN, int STAGES, bool MOE, int AROWS, class FX = NoEpilogue, bool RUNS = false>
 __global__ void __launch_bounds__(kThreads, 1)
 a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const A8W8Params p, const FX fx) {
-  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn>;
+  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn, RUNS>;
+  static_assert(!RUNS || (MOE && FX::kOn), "runs of blocks exist for the gated expert products only");
   constexpr int OW = FX::kGated ? BN / 2 : BN;  // output columns of a tile
   static_assert(OW % 32 == 0, "whole chunks of 32 output columns");
   extern __shared__ uint8_t smem_raw[];
@@ -281,7 +306,6 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int num_tiles = p.tiles_m * p.tiles_n;
   constexpr uint32_t kTmemCols = 2 * BN;
   // fused MoE: row tiles past the slots in use are skipped by every role alike
   const int rows_in_use = MOE ? __ldg(p.num_post_padded) : 0;
@@ -306,10 +330,22 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
+  int* runs = reinterpret_cast<int*>(smem + L::kRunsOff);
+  if constexpr (RUNS) {
+    if (warp == 2) {
+      const int count = find_runs(p.expert_ids, min(rows_in_use / p.block_m, fx.blocks), AROWS / p.block_m, lane, runs);
+      if (lane == 0) runs[kMaxRuns + 1] = count;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // RUNS: a tile's rows are the slots of a run of blocks, so that an expert's weights are read once for up to AROWS of its slots
+  const int tiles_m = RUNS ? runs[kMaxRuns + 1] : p.tiles_m;
+  const int num_tiles = tiles_m * p.tiles_n;
+  auto first_row = [&](int mb) { return RUNS ? runs[mb] * p.block_m : mb * tile_rows; };
+  auto block_of = [&](int mb) { return RUNS ? runs[mb] : (mb * tile_rows) / p.block_m; };
 
   if (warp == 0) {
     // ------------------------------ TMA producer ------------------------------
@@ -320,12 +356,12 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     bool ok = true;
     for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
       int mb, nb;
-      tile_coords(t, p.tiles_m, p.tiles_n, mb, nb);
-      if (MOE && mb * tile_rows >= rows_in_use) continue;
+      tile_coords(t, tiles_m, p.tiles_n, mb, nb);
+      if (MOE && !RUNS && mb * tile_rows >= rows_in_use) continue;
       // fused MoE: the tile's weights are rows [e * N + nb * BN, ...) of the expert stack
       int weight_rows = p.N;  // of one expert
       if constexpr (FX::kOn) weight_rows = fx.rows;
-      const int b_row = nb * OW + (MOE ? __ldg(p.expert_ids + (mb * tile_rows) / p.block_m) * weight_rows : 0);
+      const int b_row = nb * OW + (MOE ? __ldg(p.expert_ids + block_of(mb)) * weight_rows : 0);
       for (int kb = 0; kb < p.k_blocks; ++kb) {
         ok = mbar_wait_bounded(&empty_bar[stage], phase ^ 1, abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
@@ -336,7 +372,7 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         if (leader && !(kb == p.skip_kb && t == int(blockIdx.x))) {  // (test hook: one K block's loads left out)
           uint8_t* sa = smem + stage * L::kStageBytes;
           mbar_expect_tx(&full_bar[stage], L::kStageBytes);
-          tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * kBK, mb * tile_rows);
+          tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * kBK, first_row(mb));
           tma_load_2d(sa + L::kABytes, &tmap_b, &full_bar[stage], kb * kBK, b_row);
           if (FX::kGated) tma_load_2d(sa + L::kABytes + OW * kBK, &tmap_b, &full_bar[stage], kb * kBK, b_row + p.N);
           ++issued;
@@ -366,9 +402,9 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     bool ok = true;
     bool issued_any = false;
     for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
-      if (MOE) {
+      if (MOE && !RUNS) {
         int mb, nb;
-        tile_coords(t, p.tiles_m, p.tiles_n, mb, nb);
+        tile_coords(t, tiles_m, p.tiles_n, mb, nb);
         if (mb * tile_rows >= rows_in_use) continue;
       }
       const int buf = local & 1;
@@ -426,18 +462,18 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     bool ok = true;
     for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
       int mb, nb;
-      tile_coords(t, p.tiles_m, p.tiles_n, mb, nb);
-      if (MOE && mb * tile_rows >= rows_in_use) continue;
+      tile_coords(t, tiles_m, p.tiles_n, mb, nb);
+      if (MOE && !RUNS && mb * tile_rows >= rows_in_use) continue;
       const int buf = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       ++local;
-      const int row = mb * tile_rows + quarter * 32 + lane;
+      const int row = first_row(mb) + quarter * 32 + lane;
       const int n0 = nb * OW;
       // column scales of this tile -> this warp's smem copy (fp32); row scale -> register
       int64_t col_base = 0;
       bool expert_ok = true;
       if (MOE) {
-        const int e = __ldg(p.expert_ids + (mb * tile_rows) / p.block_m);
+        const int e = __ldg(p.expert_ids + block_of(mb));
         if constexpr (FX::kOn) expert_ok = unsigned(e) < unsigned(fx.experts);
         col_base = expert_ok ? int64_t(e) * p.col_stride_e : 0;
       }
@@ -445,7 +481,7 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
       float rs = 0.f, rw = 1.f;
       int64_t out_row = -1;  // fused MoE: the flat (token, choice) index this slot writes, or -1
       if (MOE) {
-        if (quarter * 32 + lane < tile_rows) {
+        if (quarter * 32 + lane < (RUNS ? (runs[mb + 1] - runs[mb]) * p.block_m : tile_rows)) {
           const int flat = __ldg(p.sorted_ids + row);
           if (flat >= 0 && flat < p.num_valid && expert_ok) {
             out_row = flat;
@@ -1283,12 +1319,12 @@ __global__ void moe_gather_rows_kernel(const int8_t* __restrict__ a, int64_t lda
   for (int i = lane; i < K / 16; i += 32) dst[i] = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
 }
 
-template <typename OutT, int BN, int STAGES, int AROWS, class FX>
+template <typename OutT, int BN, int STAGES, int AROWS, class FX, bool RUNS = false>
 int launch_moe(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A8W8Params p, const FX& fx, cudaStream_t st) {
-  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn>;
+  using L = SmemLayout<BN, STAGES, AROWS, FX::kOn, RUNS>;
   constexpr int OW = FX::kGated ? BN / 2 : BN;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
-  auto kern = a8w8_umma_kernel<OutT, BN, STAGES, true, AROWS, FX>;
+  auto kern = a8w8_umma_kernel<OutT, BN, STAGES, true, AROWS, FX, RUNS>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];  // per device, so that a failure is reported on every call and not only the first
   int dev = 0;
@@ -1318,6 +1354,14 @@ int launch_moe_rows(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t
   if (p.tile_rows <= 16) return launch_moe<OutT, BN, kBudget / ((16 + BN) * kBK), 16>(a_sorted, EM, b, E, p, fx, st);
   if (p.tile_rows <= 64) return launch_moe<OutT, BN, kBudget / ((64 + BN) * kBK), 64>(a_sorted, EM, b, E, p, fx, st);
   return launch_moe<OutT, BN, kBudget / ((kBM + BN) * kBK) < 8 ? kBudget / ((kBM + BN) * kBK) : 8, kBM>(a_sorted, EM, b, E, p, fx, st);
+}
+
+// Small blocks gathered into runs of up to `rows` slots of one expert.
+template <typename OutT, int BN, class FX>
+int launch_moe_runs(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, const A8W8Params& p, int rows, cudaStream_t st, const FX& fx) {
+  constexpr int kBudget = 210 * 1024;
+  if (rows <= 64) return launch_moe<OutT, BN, kBudget / ((64 + BN) * kBK), 64, FX, true>(a_sorted, EM, b, E, p, fx, st);
+  return launch_moe<OutT, BN, kBudget / ((kBM + BN) * kBK) < 8 ? kBudget / ((kBM + BN) * kBK) : 8, kBM, FX, true>(a_sorted, EM, b, E, p, fx, st);
 }
 
 // Blocks of 256 sorted slots (or a multiple): one block is one 256-row tile of the CTA-pair kernel.

@@ -25,7 +25,7 @@ template <bool GATED> struct FusedEpilogue {
   int64_t ldr;
   int bias_dtype, act;   // act: fnn_activation
   int rows;              // weight rows (of one expert): N, or 2 N with a gate
-  int experts;           // fused MoE: slots of a block whose expert is not one of these write nothing
+  int experts, blocks;   // fused MoE: slots of a block whose expert is not one of `experts` write nothing; blocks of the slot list
 };
 
 // The hardware's 2^v and reciprocal as they are (subnormal results flushed to 0): one instruction each, where __expf and

@@ -70,7 +70,7 @@ int run_fused(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, const 
               const void* residual, int64_t ldr, int out_dtype, cudaStream_t st) {
   FusedEpilogue<GATED> fx;
   fx.bias = bias; fx.residual = residual; fx.ldr = ldr; fx.bias_dtype = bias_dtype; fx.act = act;
-  fx.rows = GATED ? 2 * p.N : p.N; fx.experts = 0;
+  fx.rows = GATED ? 2 * p.N : p.N; fx.experts = fx.blocks = 0;
   if (out_dtype == FNN_F16) return dispatch_fused<__half>(a, lda, b, ldb, p, fx, st);
   return dispatch_fused<__nv_bfloat16>(a, lda, b, ldb, p, fx, st);
 }

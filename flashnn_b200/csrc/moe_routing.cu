@@ -783,10 +783,10 @@ int launch_route(const RouteParams& p, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // One cluster does it in one launch.  Its warps take consecutive pieces of the list.  Pass 1 counts each warp's experts in
 // shared memory; prefix sums over a CTA's warps, over the cluster's CTAs (through distributed shared memory) and over the
-// experts' padded sizes give every warp its first slot of every expert; pass 2 hands the slots out in list order.  A vote
-// per bit of the expert ranks equal ones within a warp: match.any takes about 100 cycles for 32 different values, and with it the
-// list of 131072 choices took 25 us, ... with votes.  No atomics decide an order: the list is the same every time.
-constexpr int kSortThreads = 1024;
+// experts' padded sizes give every warp its first slot of every expert; pass 2 hands the slots out in list order, equal experts
+// within a warp ranked by a vote per bit of the expert (match.any takes about 100 cycles for 32 different values: 131072 choices 25 us with it, 17 with
+// votes, eight CTAs each).  No atomics decide an order: the list is the same every time.
+constexpr int kSortThreads = 1024;  // most
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kHeld = 16;
 constexpr unsigned kNoExpert = 0xffffffffu;
@@ -801,8 +801,9 @@ struct SortParams {
 };
 
 __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams p) {
-  extern __shared__ int32_t cnt[];            // [kSortWarps][E]: counts, then the warp's next slot within the expert
-  int32_t* total = cnt + kSortWarps * p.E;    // [E] this CTA's counts
+  extern __shared__ int32_t cnt[];            // [cta_warps][E]: counts, then the warp's next slot within the expert
+  const int threads = int(blockDim.x), cta_warps = threads >> 5;  // (at least one thread per expert)
+  int32_t* total = cnt + cta_warps * p.E;     // [E] this CTA's counts
   int32_t* begin = total + p.E;               // [E] first slot of the expert
   int32_t* count = begin + p.E;               // [E] slots in use of the expert
   int32_t* base = count + p.E;                // [E] first slot of the expert that is this CTA's
@@ -810,14 +811,14 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = int(cluster.block_rank()), ctas = int(cluster.num_blocks());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gw = rank * kSortWarps + warp, warps = ctas * kSortWarps;
+  const int gw = rank * cta_warps + warp, warps = ctas * cta_warps;
   const int piece = ((p.choices + warps - 1) / warps + 31) / 32 * 32;
   const int64_t lo64 = int64_t(gw) * piece;
   const int lo = int(lo64 < p.choices ? lo64 : p.choices);
   const int hi = int(lo64 + piece < p.choices ? lo64 + piece : p.choices);
   int32_t* mine = cnt + warp * p.E;
 
-  // experts of the piece's first kHeld steps stay in registers between the passes (all of it up to 131072 choices on eight CTAs)
+  // experts of the piece's first kHeld steps stay in registers between the passes (all of it up to 131072 choices)
   auto expert_of = [&](int i) {
     const unsigned x = i < hi ? unsigned(__ldg(p.ids + i)) - unsigned(p.first) : kNoExpert;
     return x < unsigned(p.E) ? x : kNoExpert;
@@ -825,7 +826,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   unsigned held[kHeld];
 #pragma unroll
   for (int s = 0; s < kHeld; ++s) held[s] = expert_of(lo + s * 32 + lane);
-  for (int i = threadIdx.x; i < kSortWarps * p.E; i += kSortThreads) cnt[i] = 0;
+  for (int i = threadIdx.x; i < cta_warps * p.E; i += threads) cnt[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int s = 0; s < kHeld; ++s)
@@ -837,22 +838,24 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   __syncthreads();
   const int e = threadIdx.x;
   if (e < p.E) {
-    int t[kSortWarps];
-#pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) t[w] = cnt[w * p.E + e];
     int run = 0;
+    for (int w0 = 0; w0 < cta_warps; w0 += 8) {
+      int t[8];
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      cnt[w * p.E + e] = run;
-      run += t[w];
+      for (int w = 0; w < 8; ++w) t[w] = w0 + w < cta_warps ? cnt[(w0 + w) * p.E + e] : 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if (w0 + w < cta_warps) cnt[(w0 + w) * p.E + e] = run;
+        run += t[w];
+      }
     }
     total[e] = run;
   }
-  cluster.sync();
+  if (ctas > 1) cluster.sync();
   int before = 0, all = 0;
   if (e < p.E) {
     for (int c = 0; c < ctas; ++c) {
-      const int t = cluster.map_shared_rank(total, c)[e];
+      const int t = ctas > 1 ? cluster.map_shared_rank(total, c)[e] : total[e];
       if (c < rank) before += t;
       all += t;
     }
@@ -867,7 +870,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
   if (lane == 31) scan[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    int t = scan[lane];
+    int t = lane < cta_warps ? scan[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, t, o);
@@ -876,7 +879,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
     scan[lane] = t;
   }
   __syncthreads();
-  const int in_use = scan[kSortWarps - 1];
+  const int in_use = scan[cta_warps - 1];
   const int start = sum - padded + (warp > 0 ? scan[warp - 1] : 0);
   if (e < p.E) {
     begin[e] = start;
@@ -912,9 +915,9 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortParams
     for (int s = b + n + lane; s < end; s += 32) p.sorted[s] = p.choices;
     for (int k = b / p.bm + lane; k < end / p.bm; k += 32) p.experts[k] = x;
   }
-  for (int s = in_use + rank * kSortThreads + threadIdx.x; s < p.slots; s += ctas * kSortThreads) p.sorted[s] = p.choices;
-  for (int k = in_use / p.bm + rank * kSortThreads + threadIdx.x; k < p.slots / p.bm; k += ctas * kSortThreads) p.experts[k] = 0;
-  cluster.sync();  // nobody leaves while another CTA may still read its counts
+  for (int s = in_use + rank * threads + threadIdx.x; s < p.slots; s += ctas * threads) p.sorted[s] = p.choices;
+  for (int k = in_use / p.bm + rank * threads + threadIdx.x; k < p.slots / p.bm; k += ctas * threads) p.experts[k] = 0;
+  if (ctas > 1) cluster.sync();  // nobody leaves while another CTA may still read its counts
 }
 
 // ---------------------------------------------------------------------------
@@ -1030,7 +1033,6 @@ extern "C" int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_
   if (!num_tokens_post_padded || (num_choices > 0 && (!topk_ids || !sorted_token_ids || !expert_ids)))
     return fail(FNN_ERR_NULL_POINTER, "moe_sort: null tensor pointer");
   SortParams p{topk_ids, sorted_token_ids, expert_ids, num_tokens_post_padded, int(num_choices), int(E), block_m, int(first_expert), int(EM)};
-  const size_t smem = size_t(kSortWarps + 4) * size_t(E) * sizeof(int32_t);
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
@@ -1038,13 +1040,21 @@ extern "C" int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_
   dev &= 63;
   std::call_once(once[dev], [&] {
     attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortWarps + 4) * kSortMaxExperts * 4);
+    if (attr_err[dev] == cudaSuccess) attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   });
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(moe_sort)");
   cudaLaunchConfig_t cfg = {};
-  const unsigned ctas = num_choices > 4096 ? 8u : 1u;
+  // One CTA where a launch is all there is to it, else as many as a cluster holds: they write the slots, padding included, and 16 SMs
+  // write them faster than one.  Measured, one CTA / a cluster: 64 tokens x 2 of 8 experts (240 slots) 4.4 / 5.4 us, 512 x 2 of 8
+  // in blocks of 128 (1920) 5.3 / 5.6, 2048 x 2 of 8 (4992) 7.9 / 5.8, 64 x 8 of 256 (32768) 18 / 6.7.  A cluster of 8: 131072
+  // choices 16.8 us, of 16: 12.1.  Warps cost barriers, and pay where their steps (32 choices each) are many: 512 / 1024
+  // threads a CTA, 16384 choices 7.4 / 8.7 us, 131072 12.1 / 12.7, 262144 22.9 / 17.8.
+  const unsigned ctas = need > 2048 ? 16u : 1u;
+  unsigned threads = ctas == 1 ? 256u : num_choices > 131072 ? unsigned(kSortThreads) : 512u;
+  if (int64_t(threads) < E) threads = unsigned((E + 31) / 32 * 32);
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = size_t(threads / 32 + 4) * size_t(E) * sizeof(int32_t);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -67,6 +67,10 @@ struct A8W8Params {
   int sk_tiles, sk_units, sk_tail_units, sk_slots;  // sk_slots: slots reserved per tail-sharing pair
 };
 
+// The gated expert products start while the gather of their token rows still runs (programmatic stream serialisation): everything
+// but those rows was complete before the gather began, so only the producer waits, with the first weights already on their way.
+__device__ __forceinline__ void wait_for_gather() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 constexpr int kMaxRuns = 1024;  // blocks of a slot list that can be gathered into runs
 
 // Runs of consecutive blocks of one expert, at most `most` blocks long: runs[i] becomes run i's first block, runs[count] the number
@@ -372,9 +376,10 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         if (leader && !(kb == p.skip_kb && t == int(blockIdx.x))) {  // (test hook: one K block's loads left out)
           uint8_t* sa = smem + stage * L::kStageBytes;
           mbar_expect_tx(&full_bar[stage], L::kStageBytes);
-          tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * kBK, first_row(mb));
           tma_load_2d(sa + L::kABytes, &tmap_b, &full_bar[stage], kb * kBK, b_row);
           if (FX::kGated) tma_load_2d(sa + L::kABytes + OW * kBK, &tmap_b, &full_bar[stage], kb * kBK, b_row + p.N);
+          if (MOE && FX::kOn && issued == 0) wait_for_gather();
+          tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * kBK, first_row(mb));
           ++issued;
         }
         __syncwarp();
@@ -758,8 +763,9 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           uint8_t* sa = smem + stage * L::kStageBytes;
           const uint32_t full_in_leader = map_to_cta(smem_u32(&full_bar[stage]), 0);
           if (rank == 0) mbar_expect_tx(&full_bar[stage], 2 * L::kStageBytes);
-          tma_load_2d_pair(sa, &tmap_a, full_in_leader, kb * kBK, mb * 256 + int(rank) * 128);
           tma_load_2d_pair(sa + L::kABytes, &tmap_b, full_in_leader, kb * kBK, b_row);
+          if (MOE && FX::kOn && issued == 0) wait_for_gather();
+          tma_load_2d_pair(sa, &tmap_a, full_in_leader, kb * kBK, mb * 256 + int(rank) * 128);
           ++issued;
         }
         __syncwarp();
@@ -1309,6 +1315,7 @@ inline A8W8Plan plan_a8w8(int M, int N, int sms, bool gated) {
 __global__ void moe_gather_rows_kernel(const int8_t* __restrict__ a, int64_t lda, const int32_t* __restrict__ sorted_ids,
                                        const int32_t* __restrict__ num_post_padded, int num_valid, int top_k,
                                        int8_t* __restrict__ a_sorted, int K, int EM) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (for a product that was launched to overlap, see wait_for_gather)
   const int slot = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (slot >= EM || slot >= __ldg(num_post_padded)) return;
   const int lane = threadIdx.x & 31;
@@ -1317,6 +1324,21 @@ __global__ void moe_gather_rows_kernel(const int8_t* __restrict__ a, int64_t lda
   const uint4* src = reinterpret_cast<const uint4*>(a + int64_t(valid ? flat / top_k : 0) * lda);
   uint4* dst = reinterpret_cast<uint4*>(a_sorted + int64_t(slot) * K);
   for (int i = lane; i < K / 16; i += 32) dst[i] = valid ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+}
+
+template <class K, class... Args>
+int launch_overlapped(K kern, unsigned grid, int threads, size_t smem, cudaStream_t st, const char* what, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
 }
 
 template <typename OutT, int BN, int STAGES, int AROWS, class FX, bool RUNS = false>
@@ -1344,6 +1366,7 @@ int launch_moe(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t E, A
   p.k_blocks = (p.K + kBK - 1) / kBK;
   const int tiles = p.tiles_m * p.tiles_n;
   const int grid = tiles < sm_count() ? tiles : sm_count();
+  if constexpr (FX::kOn) return launch_overlapped(kern, unsigned(grid), kThreads, L::kDynamicBytes, st, "fused moe a8w8 gated launch", ta, tb, p, fx);
   kern<<<grid, kThreads, L::kDynamicBytes, st>>>(ta, tb, p, fx);
   return check_cuda(cudaGetLastError(), "fused moe a8w8 launch");
 }
@@ -1394,6 +1417,8 @@ int launch_moe_pair(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t
   p.out_tma = 0;
   const int tiles = p.tiles_m * p.tiles_n;
   const int pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
+  if constexpr (FX::kOn)
+    return launch_overlapped(kern, unsigned(2 * pairs), (2 + EPI) * 32, L::kDynamicBytes, st, "fused moe a8w8 gated (CTA pair) launch", ta, tb, ta, p, fx);
   kern<<<2 * pairs, (2 + EPI) * 32, L::kDynamicBytes, st>>>(ta, tb, ta, p, fx);
   return check_cuda(cudaGetLastError(), "fused moe a8w8 (CTA pair) launch");
 }

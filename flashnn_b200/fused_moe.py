@@ -5,7 +5,7 @@ with per-channel or per-group scales), optionally scaled by the routing weight, 
 import torch
 
 from . import _lib
-from .quant_gemm import _DT, _flat, _on_device, _one_device, _require_cuda, _stream, _workspace
+from .quant_gemm import _DT, _flat, _launch, _on_device, _one_device, _require_cuda, _stream, _workspace
 
 
 def _i32(t: torch.Tensor) -> torch.Tensor:
@@ -57,42 +57,51 @@ def fused_moe_a8w8_gated_forward(A, B, C, alpha_row_ptr, alpha_col_ptr, topk_ids
     multiplies; C [M, top_k, N] fp16/bf16 (written in place, rows named by no slot are left alone); alpha_row_ptr [M];
     alpha_col_ptr [E, 2 N]; bias None or [E, 2 N]; sorted_token_ids [EM], expert_ids [EM / BM] and num_tokens_post_padded [1]
     as `moe_sort_tokens` gives them; activation "none", "relu", "sigmoid", "silu", "gelu" or "gelu_tanh"."""
-    _one_device(A, B, C, alpha_row_ptr, alpha_col_ptr, bias, sorted_token_ids, expert_ids, num_tokens_post_padded)
-    assert activation in _lib.ACTIVATIONS, f"unknown activation {activation!r}"
-    assert sorted_token_ids.stride(0) == 1
-    assert B.dim() == 3 and B.shape[1] % 2 == 0, "B must be [E, 2 N, K]"
-    assert A.dtype == torch.int8 and B.dtype == torch.int8, "A and B must be int8"
-    assert A.shape[-1] == B.shape[2], "A and B must have the same K"
-    assert C.dtype in (torch.float16, torch.bfloat16) and C.dim() == 3 and (C.shape[2] <= 1 or C.stride(2) == 1)
+    index = _one_device(A, B, C, alpha_row_ptr, alpha_col_ptr, bias, sorted_token_ids, expert_ids, num_tokens_post_padded)
+    act = _lib.ACTIVATIONS.get(activation)
+    assert act is not None, f"unknown activation {activation!r}"
+    assert B.dim() == 3 and C.dim() == 3, "B must be [E, 2 N, K] and C [M, top_k, N]"
     E, R, K = B.shape
     top_k, BM = int(top_k), int(BM)
+    assert R % 2 == 0, "B must be [E, 2 N, K]"
+    assert A.dtype == torch.int8 and B.dtype == torch.int8, "A and B must be int8"
+    assert A.shape[-1] == K, "A and B must have the same K"
+    c_dt = _DT.get(C.dtype)
+    assert c_dt is not None and c_dt != _lib.F32, "C must be float16 or bfloat16"
     M, N = A.numel() // K if K else 0, R // 2
     assert C.shape == (M, top_k, N), "C must be [M, top_k, N]"
     assert topk_ids.numel() == M * top_k, "topk_ids must be [M, top_k]"
     if C.numel() == 0:
         return C
-    ldo = C.stride(1) if top_k > 1 else C.stride(0) if M > 1 else N
-    assert top_k <= 1 or M <= 1 or C.stride(0) == top_k * C.stride(1), "C must be viewable as [M * top_k, N]"
-    a2 = A if A.dim() == 2 else A.reshape(-1, K)
-    if a2.stride(1) != 1:
-        a2 = a2.contiguous()
-    row = _flat(alpha_row_ptr)
-    assert row.numel() == M and row.dtype in _DT, "alpha_row_ptr must be [M] in a float dtype"
-    assert alpha_col_ptr.numel() == E * R and alpha_col_ptr.dtype in _DT, "alpha_col_ptr must be [E, 2 N] in a float dtype"
-    assert bias is None or (bias.numel() == E * R and bias.dtype in _DT), "bias must be [E, 2 N] in a float dtype"
-    assert expert_ids.numel() * BM >= sorted_token_ids.numel(), "expert_ids must be [EM / BM]"
-    b, col = B.contiguous(), alpha_col_ptr.contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    sid, eid, npp = _i32(sorted_token_ids), _i32(expert_ids).contiguous(), _i32(num_tokens_post_padded)
-    with _on_device(A):
-        L = _lib.lib()
-        need = L.fnn_fused_moe_a8w8_workspace_bytes(sid.shape[0], K)
-        ws = A.new_empty(max(need, 1))
-        _lib.check(L.fnn_fused_moe_a8w8_gated(
-            a2.data_ptr(), a2.stride(0) if M > 1 else K, b.data_ptr(), E, N, K, row.data_ptr(), _DT[row.dtype], col.data_ptr(),
-            _DT[col.dtype], bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0,
-            _lib.ACTIVATIONS[activation], sid.data_ptr(), sid.shape[0], eid.data_ptr(), npp.data_ptr(), M * top_k,
-            top_k, BM, C.data_ptr(), _DT[C.dtype], ldo, ws.data_ptr(), need, _stream(A)))
+    ldo = N
+    if not C.is_contiguous():
+        assert N <= 1 or C.stride(2) == 1, "C must be contiguous along N"
+        assert top_k <= 1 or M <= 1 or C.stride(0) == top_k * C.stride(1), "C must be viewable as [M * top_k, N]"
+        ldo = C.stride(1) if top_k > 1 else C.stride(0) if M > 1 else N
+    a2, lda = (A if A.dim() == 2 else A.reshape(-1, K)), K
+    if not a2.is_contiguous():
+        if K > 1 and a2.stride(1) != 1 or M > 1 and a2.stride(0) < K:  # (or a broadcast one)
+            a2 = a2.contiguous()
+        elif M > 1:
+            lda = a2.stride(0)
+    row, col, b = _flat(alpha_row_ptr), alpha_col_ptr.contiguous(), B.contiguous()
+    row_dt, col_dt = _DT.get(row.dtype), _DT.get(col.dtype)
+    assert row.numel() == M and row_dt is not None, "alpha_row_ptr must be [M] in a float dtype"
+    assert col.numel() == E * R and col_dt is not None, "alpha_col_ptr must be [E, 2 N] in a float dtype"
+    bias_ptr, bias_dt = None, 0
+    if bias is not None:
+        bias, bias_dt = bias.contiguous(), _DT.get(bias.dtype)
+        assert bias.numel() == E * R and bias_dt is not None, "bias must be [E, 2 N] in a float dtype"
+        bias_ptr = bias.data_ptr()
+    sid, eid, npp = _i32(sorted_token_ids).contiguous(), _i32(expert_ids).contiguous(), _i32(num_tokens_post_padded)
+    em = sid.numel()
+    assert BM >= 1 and eid.numel() * BM >= em, "expert_ids must be [EM / BM]"
+    # (a workspace of its own for every call: the allocator keeps streams and captured graphs apart)
+    need = (em * K + 255) // 256 * 256
+    ws = A.new_empty(need)
+    _launch(index, _lib.lib().fnn_fused_moe_a8w8_gated, a2.data_ptr(), lda, b.data_ptr(), E, N, K, row.data_ptr(), row_dt,
+            col.data_ptr(), col_dt, bias_ptr, bias_dt, act, sid.data_ptr(), em, eid.data_ptr(), npp.data_ptr(), M * top_k, top_k, BM,
+            C.data_ptr(), c_dt, ldo, ws.data_ptr(), need)
     return C
 
 

@@ -5,9 +5,13 @@ token's choices."""
 import torch
 
 from . import _lib
-from .fused_moe import _i32
 from .kernel_backend import BackendKernel
-from .quant_gemm import _DT, _flat, _on_device, _one_device, _stream
+from .quant_gemm import _DT, _flat, _launch, _one_device
+
+
+def _ids32(t):
+    """Expert numbers as int32; what does not fit stays outside every range of experts."""
+    return t if t.dtype == torch.int32 else t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
 
 
 class MoeRouting(BackendKernel):
@@ -31,25 +35,29 @@ class MoeRouting(BackendKernel):
         self.num_experts, self.top_k = num_experts, top_k
         self.scoring, self.renormalize, self.scale = scoring, bool(renormalize), float(scale)
         self.num_groups, self.topk_groups, self.group_score = num_groups, topk_groups, group_score
+        self._scoring, self._group_score = _lib.SCORINGS[scoring], _lib.GROUP_SCORES[group_score]
 
     def _cuda_impl(self, logits, bias=None):
-        _one_device(logits, bias)
+        index = _one_device(logits, bias)
         assert logits.dim() == 2 and logits.shape[1] == self.num_experts, "logits must be [M, num_experts]"
-        assert logits.dtype in _DT, "logits must be float16, bfloat16 or float32"
+        dt = _DT.get(logits.dtype)
+        assert dt is not None, "logits must be float16, bfloat16 or float32"
         m, e = logits.shape
-        if e > 1 and logits.stride(1) != 1:
-            logits = logits.contiguous()
+        ldl = e
+        if not logits.is_contiguous():
+            if e > 1 and logits.stride(1) != 1 or m > 1 and logits.stride(0) < e:  # (or a broadcast one)
+                logits = logits.contiguous()
+            elif m > 1:
+                ldl = logits.stride(0)
+        bias_ptr = None
         if bias is not None:
             assert bias.numel() == e and bias.is_floating_point(), "bias must be [num_experts]"
             bias = _flat(bias if bias.dtype == torch.float32 else bias.float())
+            bias_ptr = bias.data_ptr()
         weights = logits.new_empty((m, self.top_k), dtype=torch.float32)
         ids = logits.new_empty((m, self.top_k), dtype=torch.int32)
-        with _on_device(logits):
-            _lib.check(_lib.lib().fnn_moe_route(
-                logits.data_ptr(), _DT[logits.dtype], logits.stride(0) if m > 1 else e, m, e,
-                bias.data_ptr() if bias is not None else None, _lib.SCORINGS[self.scoring], int(self.renormalize),
-                self.num_groups, self.topk_groups, _lib.GROUP_SCORES[self.group_score], self.scale, self.top_k,
-                weights.data_ptr(), ids.data_ptr(), _stream(logits)))
+        _launch(index, _lib.lib().fnn_moe_route, logits.data_ptr(), dt, ldl, m, e, bias_ptr, self._scoring, self.renormalize,
+                self.num_groups, self.topk_groups, self._group_score, self.scale, self.top_k, weights.data_ptr(), ids.data_ptr())
         return weights, ids
 
     def forward(self, logits, bias=None):
@@ -63,17 +71,21 @@ def moe_sort_tokens(topk_ids, num_experts, BM, first_expert=0):
     Experts are first_expert .. first_expert + num_experts - 1 and numbered from 0 in expert_ids; a choice of any other
     expert (one of another device, or -1) gets no slot.  EM depends on the sizes alone: the most slots that any choice of
     experts fills."""
-    _one_device(topk_ids)
+    index = _one_device(topk_ids)
     assert topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64"
     assert num_experts >= 1 and BM >= 1, "num_experts and BM must be positive"
-    ids = _i32(topk_ids).contiguous()
-    L = _lib.lib()
-    em = L.fnn_moe_sort_slots(ids.numel(), num_experts, BM)
+    assert first_expert >= 0, "first_expert must not be negative"
+    ids = _ids32(topk_ids)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    n = ids.numel()
+    used = min(n, num_experts)
+    blocks = used + (n - used) // BM  # fnn_moe_sort_slots
+    em = blocks * BM
     # one allocation, three views
-    sorted_ids, experts, in_use = ids.new_empty(em + em // BM + 1).split((em, em // BM, 1))
-    with _on_device(ids):
-        _lib.check(L.fnn_moe_sort(ids.data_ptr(), ids.numel(), num_experts, first_expert, BM, sorted_ids.data_ptr(), em,
-                                  experts.data_ptr(), in_use.data_ptr(), _stream(ids)))
+    sorted_ids, experts, in_use = ids.new_empty(em + blocks + 1).split((em, blocks, 1))
+    _launch(index, _lib.lib().fnn_moe_sort, ids.data_ptr(), n, num_experts, first_expert, BM, sorted_ids.data_ptr(), em,
+            experts.data_ptr(), in_use.data_ptr())
     return sorted_ids, experts, in_use
 
 
@@ -83,30 +95,42 @@ def moe_combine(C, topk_weights=None, topk_ids=None, num_experts=None, first_exp
 
     With topk_ids [M, top_k] choices of experts outside first_expert .. first_expert + num_experts - 1 are left out: the
     expert products did not write their rows of C, which are not read."""
-    _one_device(C, topk_weights, topk_ids, residual)
-    assert C.dim() == 3 and C.dtype in (torch.float16, torch.bfloat16), "C must be [M, top_k, N] in float16 or bfloat16"
+    index = _one_device(C, topk_weights, topk_ids, residual)
+    dt = _DT.get(C.dtype)
+    assert C.dim() == 3 and dt is not None and dt != _lib.F32, "C must be [M, top_k, N] in float16 or bfloat16"
     m, k, n = C.shape
-    if n > 1 and C.stride(2) != 1:
-        C = C.contiguous()
+    ldm, ldk = k * n, n
+    if not C.is_contiguous():
+        if n > 1 and C.stride(2) != 1:
+            C = C.contiguous()
+        else:
+            ldm, ldk = C.stride(0) if m > 1 else ldm, C.stride(1) if k > 1 else n
+    w_ptr = ids_ptr = res_ptr = None
     if topk_weights is not None:
         assert topk_weights.shape == (m, k) and topk_weights.dtype in _DT, "topk_weights must be [M, top_k] in a float dtype"
         topk_weights = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
         if not topk_weights.is_contiguous():
             topk_weights = topk_weights.contiguous()
+        w_ptr = topk_weights.data_ptr()
+    experts = 1
     if topk_ids is not None:
         assert topk_ids.shape == (m, k) and num_experts is not None and num_experts >= 1, "topk_ids must be [M, top_k], with num_experts"
-        topk_ids = _i32(topk_ids).contiguous()
-    ldr = 0
+        assert topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64"
+        assert first_expert >= 0, "first_expert must not be negative"
+        topk_ids, experts = _ids32(topk_ids), num_experts
+        if not topk_ids.is_contiguous():
+            topk_ids = topk_ids.contiguous()
+        ids_ptr = topk_ids.data_ptr()
+    ldr = n
     if residual is not None:
         assert residual.shape == (m, n) and residual.dtype == C.dtype, "residual must be [M, N] in C's dtype"
-        if n > 1 and residual.stride(1) != 1:
-            residual = residual.contiguous()
-        ldr = residual.stride(0) if m > 1 else n
+        if not residual.is_contiguous():
+            if n > 1 and residual.stride(1) != 1:
+                residual = residual.contiguous()
+            elif m > 1:
+                ldr = residual.stride(0)
+        res_ptr = residual.data_ptr()
     out = C.new_empty((m, n))
-    with _on_device(C):
-        _lib.check(_lib.lib().fnn_moe_combine(
-            C.data_ptr(), _DT[C.dtype], C.stride(0) if m > 1 else k * n, C.stride(1) if k > 1 else n, m, k, n,
-            topk_weights.data_ptr() if topk_weights is not None else None, topk_ids.data_ptr() if topk_ids is not None else None,
-            num_experts if topk_ids is not None else 1, first_expert, residual.data_ptr() if residual is not None else None, ldr,
-            out.data_ptr(), n, _stream(C)))
+    _launch(index, _lib.lib().fnn_moe_combine, C.data_ptr(), dt, ldm, ldk, m, k, n, w_ptr, ids_ptr, experts, first_expert,
+            res_ptr, ldr, out.data_ptr(), n)
     return out

@@ -64,17 +64,32 @@ def _require_cuda(*tensors):
 
 
 def _one_device(first, *others):
-    """Refuses CPU tensors and tensors of different devices (None is left out)."""
+    """The index of the one device that holds all the tensors (None is left out); refuses CPU tensors and tensors of different
+    devices."""
     index = first.get_device()
-    for t in (first, *others):
-        if t is not None and t.get_device() != index or index < 0:
-            _require_cuda(first, *others)
-            raise RuntimeError("flashnn_b200 operators need all tensors on one device")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        _require_cuda(first, *others)
+        raise RuntimeError("flashnn_b200 operators need all tensors on one device")
+    return index
 
 
 def _flat(t):
     """t as a contiguous vector; free for one (a reshape costs a microsecond)."""
     return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
+
+
+def _launch(index, entry, *args):
+    """Calls a C entry on device `index` and its current stream, and raises on a non-zero status."""
+    if torch._C._cuda_getDevice() == index:
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
 
 
 class DynamicQuantize(BackendKernel):
@@ -166,43 +181,53 @@ class GemmA8W8Epilogue(BackendKernel):
         assert activation in _lib.ACTIVATIONS, f"unknown activation {activation!r}"
         self.out_ty = out_ty
         self.activation = activation
+        self._act = _lib.ACTIVATIONS[activation]
         self.gated = bool(gated)
 
     def _cuda_impl(self, a, b, alpha_row, alpha_col, bias=None, residual=None):
-        _one_device(a, b, alpha_row, alpha_col, bias, residual)
+        index = _one_device(a, b, alpha_row, alpha_col, bias, residual)
         assert a.dim() == 2 and b.dim() == 2, "Matrix A/B must be 2-D"
         assert a.dtype == torch.int8 and b.dtype == torch.int8, "Matrix A/B must be int8 type"
-        assert self.out_ty in (torch.float16, torch.bfloat16), "Output type must be float16 or bfloat16"
-        assert a.shape[1] == b.shape[1], "Matrix B must be transposed"
-        (m, k), rows = a.shape, b.shape[0]
+        out_ty = self.out_ty
+        assert out_ty == torch.bfloat16 or out_ty == torch.float16, "Output type must be float16 or bfloat16"
+        (m, k), (rows, kb) = a.shape, b.shape
+        assert k == kb, "Matrix B must be transposed"
         assert not self.gated or rows % 2 == 0, "with a gate matrix B must have an even number of rows"
         n = rows // 2 if self.gated else rows
-        lda, ldb = (a.stride(0) if m > 1 else k), (b.stride(0) if rows > 1 else k)
-        if k > 1 and a.stride(1) != 1:
-            a, lda = a.contiguous(), k
-        if k > 1 and b.stride(1) != 1:
-            b, ldb = b.contiguous(), k
+        lda = ldb = k
+        if not a.is_contiguous():
+            if k > 1 and a.stride(1) != 1 or m > 1 and a.stride(0) < k:  # (or a broadcast one)
+                a = a.contiguous()
+            elif m > 1:
+                lda = a.stride(0)
+        if not b.is_contiguous():
+            if k > 1 and b.stride(1) != 1 or rows > 1 and b.stride(0) < k:
+                b = b.contiguous()
+            elif rows > 1:
+                ldb = b.stride(0)
         row, col = _flat(alpha_row), _flat(alpha_col)
         assert row.numel() == m and col.numel() == rows, "scale shapes must be [M] and [N] (2 N with a gate)"
-        assert row.dtype in _DT and col.dtype in _DT, "scales must be float16, bfloat16 or float32"
+        row_dt, col_dt = _DT.get(row.dtype), _DT.get(col.dtype)
+        assert row_dt is not None and col_dt is not None, "scales must be float16, bfloat16 or float32"
+        bias_ptr, bias_dt = None, 0
         if bias is not None:
             bias = _flat(bias)
-            assert bias.numel() == rows and bias.dtype in _DT, "bias must be [N] (2 N with a gate) in a float dtype"
-        ldr = 0
+            bias_dt = _DT.get(bias.dtype)
+            assert bias.numel() == rows and bias_dt is not None, "bias must be [N] (2 N with a gate) in a float dtype"
+            bias_ptr = bias.data_ptr()
+        res_ptr, ldr = None, n
         if residual is not None:
-            assert residual.shape == (m, n) and residual.dtype == self.out_ty, "residual must be [M, N] in the output type"
-            if n > 1 and residual.stride(1) != 1:
-                residual = residual.contiguous()
-            ldr = residual.stride(0) if m > 1 else n
-        out = a.new_empty((m, n), dtype=self.out_ty)
-        with _on_device(a):
-            _lib.check(_lib.lib().fnn_gemm_a8w8_epilogue(
-                a.data_ptr(), lda, b.data_ptr(), ldb,
-                row.data_ptr(), _DT[row.dtype], col.data_ptr(), _DT[col.dtype],
-                bias.data_ptr() if bias is not None else None, _DT[bias.dtype] if bias is not None else 0,
-                _lib.ACTIVATIONS[self.activation], int(self.gated),
-                residual.data_ptr() if residual is not None else None, ldr,
-                out.data_ptr(), _DT[self.out_ty], n, m, n, k, _stream(a)))
+            assert residual.shape == (m, n) and residual.dtype == out_ty, "residual must be [M, N] in the output type"
+            if not residual.is_contiguous():
+                if n > 1 and residual.stride(1) != 1:
+                    residual = residual.contiguous()
+                elif m > 1:
+                    ldr = residual.stride(0)
+            res_ptr = residual.data_ptr()
+        out = a.new_empty((m, n), dtype=out_ty)
+        _launch(index, _lib.lib().fnn_gemm_a8w8_epilogue, a.data_ptr(), lda, b.data_ptr(), ldb, row.data_ptr(), row_dt,
+                col.data_ptr(), col_dt, bias_ptr, bias_dt, self._act, self.gated, res_ptr, ldr, out.data_ptr(), _DT[out_ty], n,
+                m, n, k)
         return out
 
     def forward(self, a, b, alpha_row, alpha_col, bias=None, residual=None):

@@ -131,6 +131,17 @@ def test_views_strides_and_misaligned_operands(m):
     assert torch.equal(out, run_gemm(dict(base, residual=one_row.contiguous()), "silu", True, out_ty))
 
 
+def test_broadcast_operands():
+    import flashnn_b200 as F
+    c = gemm_case(6, 520, 4096, True, False, False, torch.float16, seed=8)
+    want = run_gemm(dict(c, a=c["a"][:1].expand(6, -1).contiguous(), b=c["b"][:1].expand(1040, -1).contiguous()), "silu", True, torch.float16)
+    got = run_gemm(dict(c, a=c["a"][:1].expand(6, -1), b=c["b"][:1].expand(1040, -1)), "silu", True, torch.float16)
+    assert torch.equal(got, want)
+    x = torch.randn(1, 40, device="cuda")
+    f = F.MoeRouting(40, 4)
+    assert all(torch.equal(a, b) for a, b in zip(f(x.expand(9, -1)), f(x.expand(9, -1).contiguous())))
+
+
 def test_empty_and_degenerate_sizes():
     for m, n, k in [(0, 8, 64), (5, 0, 64)]:
         assert run_gemm(gemm_case(m, n, k, True, True, True, torch.float16), "silu", True, torch.float16).shape == (m, n)
@@ -322,6 +333,11 @@ def test_expert_sort_one_expert_takes_all_and_none_at_all():
                 assert torch.equal(got.cpu(), want)
     slots, experts, used = flashnn_b200.moe_sort_tokens(torch.zeros(0, 2, device="cuda", dtype=torch.int64), 8, 64)
     assert slots.numel() == experts.numel() == 0 and used.tolist() == [0]
+    x = torch.tensor([[-2 ** 63, 2 ** 32, 2 ** 32 + 3, 2 ** 63 - 1, 3, -1]], device="cuda")  # 64-bit numbers that are no experts
+    slots, experts, used = flashnn_b200.moe_sort_tokens(x, 8, 4)
+    assert used.tolist() == [4] and slots[:4].tolist() == [4, 6, 6, 6] and experts[0] == 3
+    c = torch.randn(1, 6, 16, device="cuda").half()
+    assert torch.equal(flashnn_b200.moe_combine(c, topk_ids=x, num_experts=8)[0], c[0, 4])
     x = torch.randint(0, 8, (50, 6), device="cuda")
     for a, b in zip(flashnn_b200.moe_sort_tokens(x[:, ::2], 8, 16), flashnn_b200.moe_sort_tokens(x[:, ::2].int().contiguous(), 8, 16)):
         assert torch.equal(a, b)

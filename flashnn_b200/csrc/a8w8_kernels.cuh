@@ -265,7 +265,7 @@ __device__ __forceinline__ void fused_chunk(const uint32_t (&r)[32], const uint3
     scale_chunk(u, rs, cs + BN / 2 + c32, same16, p, w);
     if (fx.bias) add_bias32(cs + BN + BN / 2 + c32, w);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= w[j];
+    for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], w[j]);
   }
 }
 

@@ -5,6 +5,7 @@
 //   gated   out = T(act(v[n]) * v[N + n] + r[m, n])     the weight has 2 N rows: the N rows inside the activation, then
 //                                                       the N rows that its value multiplies
 //
+// Bias, gate and residual are each rounded (__fadd_rn, __fmul_rn are never contracted), so that all kernels give the same bits.
 // The gate needs the sums of weight rows n and N + n in one thread, so a gated tile of BN accumulator columns takes
 // BN / 2 rows from each half of the weight: the two halves meet in the accumulator, and the output, half as wide as the
 // product, is all that leaves the chip.
@@ -112,15 +113,16 @@ __device__ __forceinline__ void load_residual32(const FX& fx, int row, int col0,
 template <typename T> __device__ __forceinline__ void add_residual32(const uint32_t (&r)[16], float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    v[2 * j] += lo_of<T>(r[j]);
-    v[2 * j + 1] += hi_of<T>(r[j]);
+    v[2 * j] = __fadd_rn(v[2 * j], lo_of<T>(r[j]));
+    v[2 * j + 1] = __fadd_rn(v[2 * j + 1], hi_of<T>(r[j]));
   }
 }
 __device__ __forceinline__ void add_bias32(const float* b, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 t = *reinterpret_cast<const float4*>(b + j);
-    v[j] += t.x; v[j + 1] += t.y; v[j + 2] += t.z; v[j + 3] += t.w;
+    v[j] = __fadd_rn(v[j], t.x); v[j + 1] = __fadd_rn(v[j + 1], t.y);
+    v[j + 2] = __fadd_rn(v[j + 2], t.z); v[j + 3] = __fadd_rn(v[j + 3], t.w);
   }
 }
 

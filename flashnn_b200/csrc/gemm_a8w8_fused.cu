@@ -23,13 +23,274 @@ __global__ void a8w8_fused_generic_kernel(const int8_t* __restrict__ a, int64_t 
     float s = __fmul_rn(rs, load_as_f32(p.alpha_col, p.col_dtype, row));
     if (same16) s = round_through(s, p.row_dtype);
     float v = __fmul_rn(float(acc), s);
-    if (fx.bias) v += load_as_f32(fx.bias, fx.bias_dtype, row);
+    if (fx.bias) v = __fadd_rn(v, load_as_f32(fx.bias, fx.bias_dtype, row));
     return v;
   };
   float v = activate_one(scaled(n), fx.act);
-  if (FX::kGated) v *= scaled(int64_t(p.N) + n);
-  if (fx.residual) v += to_f32(reinterpret_cast<const OutT*>(fx.residual)[m * fx.ldr + n]);
+  if (FX::kGated) v = __fmul_rn(v, scaled(int64_t(p.N) + n));
+  if (fx.residual) v = __fadd_rn(v, to_f32(reinterpret_cast<const OutT*>(fx.residual)[m * fx.ldr + n]));
   reinterpret_cast<OutT*>(p.out)[m * p.ldo + n] = from_f32<OutT>(v);
+}
+
+// ---------------------------------------------------------------------------
+// Few tiles, long K: a cluster of CTAs shares the K blocks of one 128 x 64 tile (accumulator columns).  Every CTA leaves its int32
+// sums in its shared memory; after a cluster barrier all of them take a share of the outputs, add the CTAs' sums (exact in any order)
+// through distributed shared memory and finish them, four columns a thread.  One tile per cluster, so there is nothing to
+// overlap and the epilogue can be scalar code, which is also little code: such a launch fetches every instruction once.
+// Latency bounds it: of 9 us for 16 x 4096 x 4096 the weights take 3.
+// ---------------------------------------------------------------------------
+constexpr int kSplitBN = 64;
+constexpr uint64_t kDrainNs = 2000000ull;  // for copies that are in flight when a wait has run out
+constexpr int kSplitPitch = kSplitBN + 4;  // words of a row of sums: 16-byte accesses of eight neighbouring rows hit different banks
+
+__device__ __forceinline__ int4 ld_cluster_int4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename OutT, int AROWS, int STAGES, class FX>
+__global__ void __launch_bounds__(kThreads, 1)
+a8w8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const A8W8Params p, const FX fx,
+                  const int splits) {
+  using L = SmemLayout<kSplitBN, STAGES, AROWS>;
+  constexpr int OW = FX::kGated ? kSplitBN / 2 : kSplitBN;  // output columns of a tile
+  static_assert(kBM * kSplitPitch * 4 <= STAGES * L::kStageBytes, "the sums lie where the operands were");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + STAGES;
+  uint64_t* tmem_full_bar = bars + 2 * STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmemSlotOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
+  int* sums = reinterpret_cast<int*>(smem);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(cluster_ctarank());
+  const int nb = int(blockIdx.x) / splits;
+  const int kb0 = int(int64_t(p.k_blocks) * rank / splits), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / splits);
+  const int n0 = nb * OW, rows = p.M;  // (at most 128)
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(tmem_full_bar, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kSplitBN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    const bool leader = elect_one();
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int i = kb - kb0, stage = i % STAGES;
+      ok = mbar_wait_bounded(&empty_bar[stage], uint32_t((i / STAGES) & 1) ^ 1, abort_flag, p.wait_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (leader) report(p.status, abort_flag, DEV_TIMEOUT_PRODUCER);
+        break;
+      }
+      if (leader) {
+        uint8_t* sa = smem + stage * L::kStageBytes;
+        mbar_expect_tx(&full_bar[stage], L::kStageBytes);
+        tma_load_2d(sa + L::kABytes, &tmap_b, &full_bar[stage], kb * kBK, n0);
+        if (FX::kGated) tma_load_2d(sa + L::kABytes + OW * kBK, &tmap_b, &full_bar[stage], kb * kBK, n0 + p.N);
+        tma_load_2d(sa, &tmap_a, &full_bar[stage], kb * kBK, 0);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    constexpr uint32_t idesc = umma_idesc(/*s32*/ 2, /*signed 8-bit*/ 1, kBM, kSplitBN);
+    int done = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++done) {
+      const int stage = done % STAGES;
+      bool ok = mbar_wait_bounded(&full_bar[stage], uint32_t((done / STAGES) & 1), abort_flag, p.wait_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (leader) report(p.status, abort_flag, DEV_TIMEOUT_MMA);
+        break;
+      }
+      tc_fence_after();
+      if (leader) {
+        const uint32_t sa = smem_u32(smem + stage * L::kStageBytes);
+        const uint32_t sb = sa + L::kABytes;
+#pragma unroll
+        for (int k = 0; k < kBK / kUmmaK; ++k)
+          umma_i8(tmem_base, umma_desc_k_sw128(sa + k * kUmmaK), umma_desc_k_sw128(sb + k * kUmmaK), idesc, (done | k) != 0 ? 1u : 0u);
+        tc_commit(&empty_bar[stage]);
+      }
+      __syncwarp();
+    }
+    // also after an abort: nothing is freed before the MMAs issued have completed
+    if (leader) {
+      tc_commit(tmem_full_bar);
+      int none = 0;
+      if (!mbar_wait_bounded(tmem_full_bar, 0, &none, p.wait_ns)) report(p.status, abort_flag, DEV_TIMEOUT_DRAIN);
+      // (and, after an abort, before the copies issued have landed)
+      if (*abort_flag != 0)
+        for (int i = done; i < kb1 - kb0 && i < done + STAGES; ++i) mbar_wait_bounded(&full_bar[i % STAGES], uint32_t((i / STAGES) & 1), &none, kDrainNs);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    bool ok = mbar_wait_bounded(tmem_full_bar, 0, abort_flag, p.wait_ns);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) {
+      if (lane == 0) report(p.status, abort_flag, DEV_TIMEOUT_EPILOGUE);
+    } else if (quarter * 32 < rows) {
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < kSplitBN / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32(tmem_base + (uint32_t(quarter * 32) << 16) + c * 32, r);
+        tc_wait_ld();
+        if (quarter * 32 + lane < rows) {
+          int4* dst = reinterpret_cast<int4*>(sums + (quarter * 32 + lane) * kSplitPitch + c * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dst[j] = make_int4(int(r[4 * j]), int(r[4 * j + 1]), int(r[4 * j + 2]), int(r[4 * j + 3]));
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  // a thread's outputs: four columns of a row at a time; what its first ones need from global memory is on its way during the barrier
+  struct Item {
+    float rs, cs[4], bs[4], cu[4], bu[4], res[4];
+  };
+  constexpr int kQuads = OW / 4;
+  const bool same16 = (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
+  const int items = rows * kQuads, stride = splits * kThreads;
+  auto fetch = [&](int i, Item& t) {
+    const int row = i / kQuads, col = n0 + (i % kQuads) * 4;
+    t.rs = load_as_f32(p.alpha_row, p.row_dtype, row);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool on = col + j < p.N;
+      t.cs[j] = on ? load_as_f32(p.alpha_col, p.col_dtype, col + j) : 0.f;
+      t.bs[j] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, col + j) : 0.f;
+      if (FX::kGated) {
+        t.cu[j] = on ? load_as_f32(p.alpha_col, p.col_dtype, int64_t(p.N) + col + j) : 0.f;
+        t.bu[j] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, int64_t(p.N) + col + j) : 0.f;
+      }
+      t.res[j] = (on && fx.residual) ? to_f32(reinterpret_cast<const OutT*>(fx.residual)[int64_t(row) * fx.ldr + col + j]) : 0.f;
+    }
+  };
+  int i = rank * kThreads + int(threadIdx.x);
+  Item item;
+  if (i < items) fetch(i, item);
+  __syncthreads();
+  cluster_sync_all();
+  const uint32_t sums_addr = smem_u32(sums);
+  while (i < items) {
+    const int r = i / kQuads, c = (i % kQuads) * 4;
+    int4 a = make_int4(0, 0, 0, 0), b = a;
+    for (int q = 0; q < splits; ++q) {
+      const uint32_t at = map_to_cta(sums_addr + (r * kSplitPitch + c) * 4, uint32_t(q));
+      const int4 t = ld_cluster_int4(at);
+      a.x += t.x; a.y += t.y; a.z += t.z; a.w += t.w;
+      if (FX::kGated) {
+        const int4 u = ld_cluster_int4(at + OW * 4);
+        b.x += u.x; b.y += u.y; b.z += u.z; b.w += u.w;
+      }
+    }
+    const int acc[4] = {a.x, a.y, a.z, a.w}, up[4] = {b.x, b.y, b.z, b.w};
+    auto scaled = [&](int sum, float cs, float bias) {
+      float s = __fmul_rn(item.rs, cs);
+      if (same16) s = round_through(s, p.row_dtype);
+      return __fadd_rn(__fmul_rn(float(sum), s), bias);
+    };
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = scaled(acc[j], item.cs[j], item.bs[j]);
+    activate_n(v, fx.act);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (FX::kGated) v[j] = __fmul_rn(v[j], scaled(up[j], item.cu[j], item.bu[j]));
+      v[j] = __fadd_rn(v[j], item.res[j]);
+    }
+    OutT* out = reinterpret_cast<OutT*>(p.out) + int64_t(r) * p.ldo + n0 + c;
+    if (n0 + c + 4 <= p.N && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2<OutT>(v[0], v[1]), pack2<OutT>(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + c + j < p.N) out[j] = from_f32<OutT>(v[j]);
+    }
+    i += stride;
+    if (i < items) fetch(i, item);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // nobody leaves while another CTA may still read its sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kSplitBN);
+  }
+}
+
+template <typename OutT, int AROWS, class FX>
+int launch_split(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8Params p, const FX& fx, int splits, cudaStream_t st) {
+  constexpr int kFit = 210 * 1024 / ((AROWS + kSplitBN) * kBK);
+  constexpr int STAGES = kFit < 12 ? kFit : 12;
+  using L = SmemLayout<kSplitBN, STAGES, AROWS>;
+  static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
+  constexpr int OW = FX::kGated ? kSplitBN / 2 : kSplitBN;
+  auto kern = a8w8_split_kernel<OutT, AROWS, STAGES, FX>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];  // per device, so that a failure is reported on every call and not only the first
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev &= 63;
+  std::call_once(once[dev], [&] {
+    attr_err[dev] = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamicBytes);
+  });
+  if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(a8w8 split)");
+  CUtensorMap ta, tb;
+  if (int e = make_tmap_i8(&ta, a, p.M, p.K, lda, AROWS)) return e;
+  if (int e = make_tmap_i8(&tb, b, fx.rows, p.K, ldb, OW)) return e;
+  p.tiles_n = (p.N + OW - 1) / OW;
+  p.k_blocks = (p.K + kBK - 1) / kBK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.tiles_n * splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::kDynamicBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(splits);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tb, p, fx, splits), "a8w8 split-K launch");
+}
+
+// CTAs that share a tile of at most 128 tokens (1: no sharing): as many as leave every one an SM and four K blocks, where that gains.
+// Measured, in us: a K block takes a CTA 0.25, the barrier 1.5, a thread's four columns in the joint epilogue 1.  16 x 4096 x 4096
+// 12.2 -> 9.0, 2 x 68 x 17696 36 -> 8.7, 128 x 2048 x 8192 20 -> 12.6, 64 x 2048 x 28672 55 -> 22; 64 x 1024 x 1024 7.3 -> 9.0 and 300 x 1024 x 1024
+// 7.9 -> 13.3, which this rule leaves alone.
+inline int split_of(int M, int rows, int K, int sms) {
+  if (M > kBM) return 1;
+  const int64_t tiles = (rows + kSplitBN - 1) / kSplitBN;
+  const int k_blocks = (K + kBK - 1) / kBK;
+  for (int s = 8; s > 1; s /= 2)
+    if (tiles * s <= sms && k_blocks >= 4 * s) return k_blocks * (s - 1) * 0.25 > M * (kSplitBN / 4.0) / kThreads + 1.5 * s ? s : 1;
+  return 1;
 }
 
 template <typename OutT, class FX>
@@ -46,6 +307,11 @@ int dispatch_fused(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, c
     const int r = gemv_a8w8_imma_fused(a, lda, b, ldb, p.alpha_row, p.row_dtype, p.alpha_col, p.col_dtype, p.out,
                                        std::is_same<OutT, __half>::value ? FNN_F16 : FNN_BF16, p.ldo, p.M, p.N, p.K, fx, st);
     if (r >= 0) return r;
+  }
+  if (const int splits = split_of(p.M, fx.rows, p.K, sm_count()); splits > 1) {
+    if (p.M <= 16) return launch_split<OutT, 16>(a, lda, b, ldb, p, fx, splits, st);
+    if (p.M <= 64) return launch_split<OutT, 64>(a, lda, b, ldb, p, fx, splits, st);
+    return launch_split<OutT, 128>(a, lda, b, ldb, p, fx, splits, st);
   }
   const A8W8Plan plan = plan_a8w8(p.M, p.N, sm_count(), FX::kGated);
   if (plan.pair) {

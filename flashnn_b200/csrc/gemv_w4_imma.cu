@@ -350,7 +350,7 @@ gemv_w4_imma_kernel(const WoParams p, const int num_rg, const FX fx) {
           if (same16) sc = round_through(sc, p.row_dtype);
           float v = __fmul_rn(float(fi[row * 16 + tok]), sc);
           if constexpr (FX::kOn) {
-            if (fx.bias) v += load_as_f32(fx.bias, fx.bias_dtype, ch);
+            if (fx.bias) v = __fadd_rn(v, load_as_f32(fx.bias, fx.bias_dtype, ch));
           }
           return v;
         };
@@ -361,8 +361,8 @@ gemv_w4_imma_kernel(const WoParams p, const int num_rg, const FX fx) {
           const int ch = rg * kGroupCols + cl;
           if constexpr (FX::kOn) {
             float v = activate_one(scaled(row, tok, ch), fx.act);
-            if (FX::kGated) v *= scaled(row + 8, tok, p.N + ch);
-            if (fx.residual) v += to_f32(reinterpret_cast<const T*>(fx.residual)[int64_t(tok) * fx.ldr + ch]);
+            if (FX::kGated) v = __fmul_rn(v, scaled(row + 8, tok, p.N + ch));
+            if (fx.residual) v = __fadd_rn(v, to_f32(reinterpret_cast<const T*>(fx.residual)[int64_t(tok) * fx.ldr + ch]));
             out[int64_t(tok) * p.ldo + ch] = from_f32<T>(v);
             continue;
           }

@@ -66,6 +66,16 @@ def test_epilogue_over_shapes(shape, gated):
     check_gemm(gemm_case(m, n, k, gated, i % 3 != 0, i % 2 == 0, out_ty, seed=i), act, gated, out_ty)
 
 
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape", [(2, 68, 17696), (16, 64, 512), (5, 301, 1040), (64, 33, 4112), (100, 130, 2048), (129, 70, 4112),
+                                   (300, 100, 8192), (17, 1000, 1040), (128, 200, 28672), (1, 5, 8208)], ids=str)
+def test_epilogue_with_the_k_blocks_shared_by_a_cluster(shape, gated):
+    """Few tiles and a long K: two, four or eight CTAs per tile, uneven shares of the K blocks, ragged rows and columns."""
+    m, n, k = shape
+    for i, out_ty in enumerate(DTYPES):
+        check_gemm(gemm_case(m, n, k, gated, i == 0, i == 1, out_ty, seed=n), O.ACTIVATIONS[(n + i) % 6], gated, out_ty)
+
+
 @pytest.mark.parametrize("m", [2, 33, 260])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("act", O.ACTIVATIONS)

@@ -99,7 +99,7 @@ __device__ __forceinline__ int find_runs(const int32_t* expert_ids, int blocks, 
 // more of them.  The tensor core still reads 128 rows from the A base (what lies behind the real rows belongs to the
 // following buffers; the accumulator rows it produces are never stored), so the last stage is followed by padding.
 template <int BN, int STAGES, int AROWS = kBM, bool BIAS = false, bool RUNS = false> struct SmemLayout {
-  static constexpr int kColWords = (BIAS ? 2 : 1) * BN;  // per epilogue warp: column scales, then (fused epilogue) biases
+  static constexpr int kColWords = (BIAS ? 2 : 1) * BN;  // per epilogue warp: column scales, with a fused epilogue biases too
   static constexpr int kABytes = AROWS * kBK;
   static constexpr int kBBytes = BN * kBK;
   static constexpr int kStageBytes = kABytes + kBBytes;
@@ -149,11 +149,12 @@ __device__ __forceinline__ void store_acc_chunk(const uint32_t (&r)[32], int row
 
 // s = fl32(row scale * column scale) (rounded to the scales' dtype when both share a 16-bit one), v = fl32(acc * s):
 // four column scales per shared-memory read, two products per packed fp32 multiply
-__device__ __forceinline__ void scale_chunk(const uint32_t (&r)[32], float rs, const float* cs, bool same16,
-                                            const A8W8Params& p, float (&v)[32]) {
+template <int N>
+__device__ __forceinline__ void scale_chunk(const uint32_t (&r)[N], float rs, const float* cs, bool same16,
+                                            const A8W8Params& p, float (&v)[N]) {
   const uint64_t rs2 = pack_f32x2(rs, rs);
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     const float4 c4 = *reinterpret_cast<const float4*>(cs + j);
     float s0, s1, s2, s3;
     unpack_f32x2(fmul2_rn(rs2, pack_f32x2(c4.x, c4.y)), s0, s1);
@@ -219,70 +220,82 @@ __device__ __forceinline__ void store_chunk_moe(const uint32_t (&r)[32], int64_t
   }
 }
 
-// Column scales (and biases) of a tile's accumulator columns [j0, j0 + count) -> this warp's shared copy, as fp32.
-// Accumulator column j is weight row n0 + j; with a gate the tile's upper half of the columns are rows N + n0 + j.
-template <int BN, class FX>
-__device__ __forceinline__ void stage_columns(float* cs, int j0, int count, int n0, int64_t col_base, int lane, const A8W8Params& p,
-                                              const FX& fx) {
-  if constexpr (FX::kOn) {
-    // four columns of a lane at a time: their loads are in flight together
-    constexpr int OW = FX::kGated ? BN / 2 : BN;
-    for (int j = j0 + lane; j < j0 + count; j += 128) {
-      float s[4], b[4];
+// Fused epilogue: words of shared memory for the scales and biases of OWN output columns, laid out [scales][scales of the rows that the
+// activated value multiplies][biases][their biases] (the second and fourth with a gate only).
+template <class FX, int OWN> constexpr int fused_column_words() { return (FX::kGated ? 4 : 2) * OWN; }
+// ... of output columns [n0, n0 + count), count <= OWN; weight row n, with a gate also row N + n.  A lane's loads are in flight together.
+template <int OWN, class FX>
+__device__ __forceinline__ void stage_fused_columns(float* cs, int n0, int count, int64_t col_base, int lane, const A8W8Params& p, const FX& fx) {
+  constexpr int kHalves = FX::kGated ? 2 : 1;
+  constexpr int kAtOnce = OWN >= 128 ? 4 : (OWN + 31) / 32;
+  for (int j0 = lane; j0 < count; j0 += 32 * kAtOnce) {
+    float s[kHalves][kAtOnce], b[kHalves][kAtOnce];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = j + 32 * i, n = n0 + (c < OW ? c : c - OW);
-        const int64_t at = col_base + n + (c < OW ? 0 : p.N);
-        const bool on = c < j0 + count && n < p.N;
-        s[i] = on ? load_as_f32(p.alpha_col, p.col_dtype, at) : 0.f;
-        b[i] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, at) : 0.f;
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + 32 * i;
+        const bool on = j < count && n0 + j < p.N;
+        const int64_t at = col_base + n0 + j + (h ? p.N : 0);
+        s[h][i] = on ? load_as_f32(p.alpha_col, p.col_dtype, at) : 0.f;
+        b[h][i] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, at) : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (j + 32 * i < j0 + count) {
-          cs[j + 32 * i] = s[i];
-          cs[BN + j + 32 * i] = b[i];
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + 32 * i;
+        if (j < count) {
+          cs[h * OWN + j] = s[h][i];
+          cs[(kHalves + h) * OWN + j] = b[h][i];
         }
       }
-    }
-  } else {
-    for (int j = j0 + lane; j < j0 + count; j += 32)
-      cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
   }
 }
 
-// Fused epilogue of 32 output columns of one row up to (not including) the residual: `r` are their sums and, with a
-// gate, `u` those of the rows that the activated value multiplies; cs is this warp's staged scales and biases, c32 the
-// first output column within the tile.
-template <int BN, class FX>
-__device__ __forceinline__ void fused_chunk(const uint32_t (&r)[32], const uint32_t (&u)[32], float rs, const float* cs, int c32,
-                                            bool same16, const A8W8Params& p, const FX& fx, float (&v)[32]) {
-  scale_chunk(r, rs, cs + c32, same16, p, v);
-  if (fx.bias) add_bias32(cs + BN + c32, v);
+// Fused epilogue of N output columns of one row up to (not including) the residual: `r` are their sums and, with a gate, `u` those of
+// the rows that the activated value multiplies; j: the first of them among the OWN columns staged in cs.
+template <int OWN, int N, class FX>
+__device__ __forceinline__ void fused_chunk(const uint32_t (&r)[N], const uint32_t (&u)[N], float rs, const float* cs, int j, bool same16,
+                                            const A8W8Params& p, const FX& fx, float (&v)[N]) {
+  constexpr int kHalves = FX::kGated ? 2 : 1;
+  scale_chunk(r, rs, cs + j, same16, p, v);
+  if (fx.bias) add_bias(cs + kHalves * OWN + j, v);
   activate_n(v, fx.act);
   if constexpr (FX::kGated) {
-    float w[32];
-    scale_chunk(u, rs, cs + BN / 2 + c32, same16, p, w);
-    if (fx.bias) add_bias32(cs + BN + BN / 2 + c32, w);
+    float w[N];
+    scale_chunk(u, rs, cs + OWN + j, same16, p, w);
+    if (fx.bias) add_bias(cs + 3 * OWN + j, w);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], w[j]);
+    for (int i = 0; i < N; ++i) v[i] = __fmul_rn(v[i], w[i]);
   }
 }
 
-// 32 finished values of one output row
-template <typename OutT>
-__device__ __forceinline__ void store_values(const float (&v)[32], int64_t row, int col0, const A8W8Params& p, bool vec_ok) {
+// N finished values of one output row
+template <typename OutT, int N>
+__device__ __forceinline__ void store_values(const float (&v)[N], int64_t row, int col0, const A8W8Params& p, bool vec_ok) {
   OutT* orow = reinterpret_cast<OutT*>(p.out) + row * p.ldo + col0;
-  if (col0 + 32 <= p.N && vec_ok) {
+  if (col0 + N <= p.N && vec_ok) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8)
+    for (int j = 0; j < N; j += 8)
       *reinterpret_cast<uint4*>(orow + j) =
           make_uint4(pack2<OutT>(v[j], v[j + 1]), pack2<OutT>(v[j + 2], v[j + 3]),
                      pack2<OutT>(v[j + 4], v[j + 5]), pack2<OutT>(v[j + 6], v[j + 7]));
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < N; ++j)
       if (col0 + j < p.N) orow[j] = from_f32<OutT>(v[j]);
+  }
+}
+
+// Column scales of a tile's accumulator columns -> this warp's shared copy, as fp32.
+template <int BN, class FX>
+__device__ __forceinline__ void stage_columns(float* cs, int n0, int64_t col_base, int lane, const A8W8Params& p, const FX& fx) {
+  if constexpr (FX::kOn) {
+    constexpr int OW = FX::kGated ? BN / 2 : BN;
+    stage_fused_columns<OW>(cs, n0, OW, col_base, lane, p, fx);
+  } else {
+    for (int j = lane; j < BN; j += 32) cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
   }
 }
 
@@ -482,7 +495,7 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         if constexpr (FX::kOn) expert_ok = unsigned(e) < unsigned(fx.experts);
         col_base = expert_ok ? int64_t(e) * p.col_stride_e : 0;
       }
-      stage_columns<BN>(cs, 0, BN, n0, col_base, lane, p, fx);
+      stage_columns<BN>(cs, n0, col_base, lane, p, fx);
       float rs = 0.f, rw = 1.f;
       int64_t out_row = -1;  // fused MoE: the flat (token, choice) index this slot writes, or -1
       if (MOE) {
@@ -517,11 +530,11 @@ a8w8_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
           const int64_t to = MOE ? out_row : (row < p.M ? row : -1);
           if (to >= 0 && n0 + c * 32 < p.N) {
             float v[32];
-            fused_chunk<BN>(r, u, rs, cs, c * 32, same16, p, fx, v);
+            fused_chunk<OW>(r, u, rs, cs, c * 32, same16, p, fx, v);
             if (!MOE && fx.residual) {
               uint32_t res[16];
-              load_residual32<OutT>(fx, row, n0 + c * 32, p.M, p.N, res_vec_ok, res);
-              add_residual32<OutT>(res, v);
+              load_residual<OutT>(fx, row, n0 + c * 32, p.M, p.N, res_vec_ok, res);
+              add_residual<OutT>(res, v);
             }
             store_values<OutT>(v, to, n0 + c * 32, p, vec_ok);
           }
@@ -659,15 +672,20 @@ __device__ __forceinline__ bool flag_wait_bounded(const unsigned long long* f, u
   }
 }
 
-template <int BN, int STAGES, int EPI = 4, bool BIAS = false> struct PairSmem {
-  static constexpr int kColWords = (BIAS ? 2 : 1) * BN;  // per epilogue warp: column scales, then (fused epilogue) biases
+template <int BN, int STAGES, int EPI = 4, class FX = NoEpilogue> struct PairSmem {
+  // With 16 epilogue warps (fused epilogue) a chunk is 16 columns wide and four warps share a TMEM lane quarter.
+  static constexpr int kChunk = EPI == 16 ? 16 : 32;
+  static constexpr int kParts = EPI / 4;  // warps that share a tile's chunks
+  static constexpr int kWarpChunks = ((FX::kGated ? BN / 2 : BN) / kChunk + kParts - 1) / kParts;
+  static constexpr int kOwn = kWarpChunks * kChunk;  // output columns of an epilogue warp
+  static constexpr int kColWords = FX::kOn ? fused_column_words<FX, kOwn>() : BN;  // per epilogue warp: column scales (and biases)
   static constexpr int kBN = BN;                        // output columns of a pair tile (a multiple of 32, at most 256)
   static constexpr int kABytes = kBM * kBK;             // this CTA's 128 rows of A
   static constexpr int kBBytes = (kBN / 2) * kBK;       // this CTA's BN / 2 rows of B
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kOutOff = STAGES * kStageBytes;        // [EPI epilogue warps][2][32 rows x 64 B] output staging
   static constexpr int kOutBufs = EPI == 4 ? 2 : 1;           // staging buffers per epilogue warp
-  static constexpr int kOutBytes = EPI * kOutBufs * 2048;
+  static constexpr int kOutBytes = EPI * kOutBufs * kChunk * 64;
   static constexpr int kColScaleOff = kOutOff + kOutBytes;    // [EPI][kColWords] float
   static constexpr int kBarOff = kColScaleOff + EPI * kColWords * 4;
   static constexpr int kNumBars = 2 * STAGES + 4 + 1;
@@ -677,16 +695,129 @@ template <int BN, int STAGES, int EPI = 4, bool BIAS = false> struct PairSmem {
   static constexpr int kDynamicBytes = kTotal + 1024;
 };
 
+// The fused epilogue's warps of the CTA-pair kernel (epilogue.cuh); the tile's residual is loaded a chunk ahead and fetched into L2 a tile
+// ahead.
+template <typename OutT, int BN, class L, bool MOE, int EPI, class FX>
+__device__ __forceinline__ void pair_epilogue_fused(const CUtensorMap& tmap_out, const A8W8Params& p, const FX& fx, uint8_t* smem, uint32_t tmem_base,
+                                                    int rank, int pair_id, int num_pairs, uint64_t* tmem_full_bar, uint64_t* tmem_empty_bar,
+                                                    volatile int* abort_flag) {
+  constexpr int OW = FX::kGated ? BN / 2 : BN;
+  constexpr int CW = L::kChunk, NC = OW / CW, OWN = L::kOwn;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, ewarp = warp - int(blockDim.x / 32 - EPI);
+  const int c_begin = min(ewarp / 4 * L::kWarpChunks, NC), c_end = min(c_begin + L::kWarpChunks, NC);
+  float* cs = reinterpret_cast<float*>(smem + L::kColScaleOff) + ewarp * L::kColWords;  // this warp's columns
+  uint8_t* out_stage = smem + L::kOutOff + ewarp * (CW * 64);
+  // (the expert products take the scales' product in fp32 whatever their dtypes are)
+  const bool same16 = !MOE && (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
+  const bool vec_ok = (p.ldo % 8 == 0) && (reinterpret_cast<uintptr_t>(p.out) % 16 == 0);
+  const bool has_res = !MOE && fx.residual != nullptr;
+  const bool res_vec_ok = (fx.ldr % 8 == 0) && (reinterpret_cast<uintptr_t>(fx.residual) % 16 == 0);
+  const int my_row = rank * 128 + quarter * 32 + lane;  // this thread's row within a tile
+  PairWork<false, MOE> w(p, pair_id, num_pairs);
+  bool ok = true;
+  for (int local = 0; ok && w.next(); ++local) {
+    int mb, nb;
+    tile_coords(w.tile, p.tiles_m, p.tiles_n, mb, nb);
+    const int buf = local & 1;
+    const uint32_t acc_phase = (local >> 1) & 1;
+    const int row = mb * 256 + my_row, n0 = nb * OW;
+    int64_t col_base = 0;
+    bool expert_ok = true;
+    if (MOE) {
+      const int e = __ldg(p.expert_ids + (mb * 256) / p.block_m);
+      expert_ok = unsigned(e) < unsigned(fx.experts);
+      col_base = expert_ok ? int64_t(e) * p.col_stride_e : 0;
+    }
+    stage_fused_columns<OWN>(cs, n0 + c_begin * CW, (c_end - c_begin) * CW, col_base, lane, p, fx);
+    float rs = 0.f;
+    int64_t out_row = -1;  // the output row, or -1
+    if (MOE) {
+      const int flat = __ldg(p.sorted_ids + row);
+      if (flat >= 0 && flat < p.num_valid && expert_ok) {
+        out_row = flat;
+        rs = load_as_f32(p.alpha_row, p.row_dtype, flat / p.top_k);
+      }
+    } else if (row < p.M) {
+      out_row = row;
+      rs = load_as_f32(p.alpha_row, p.row_dtype, row);
+    }
+    uint32_t res[CW / 2];
+    if (has_res) {
+      load_residual<OutT>(fx, row, n0 + c_begin * CW, p.M, p.N, res_vec_ok, res);
+      PairWork<false, MOE> ahead = w;
+      if (ahead.next()) {
+        int mb2, nb2;
+        tile_coords(ahead.tile, p.tiles_m, p.tiles_n, mb2, nb2);
+        const int row2 = mb2 * 256 + my_row, col1 = min(nb2 * OW + c_end * CW, p.N);
+        if (row2 < p.M) {
+          const OutT* src = reinterpret_cast<const OutT*>(fx.residual) + int64_t(row2) * fx.ldr;
+          for (int c = nb2 * OW + c_begin * CW; c < col1; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
+        }
+      }
+    }
+    __syncwarp();
+
+    ok = mbar_wait_bounded(&tmem_full_bar[buf], acc_phase, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) {
+      if (lane == 0) report(p.status, abort_flag, DEV_TIMEOUT_EPILOGUE);
+      break;
+    }
+    tc_fence_after();
+    const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + buf * 256;
+#pragma unroll 1
+    for (int c = c_begin; c < c_end; ++c) {
+      const int col0 = n0 + c * CW;
+      uint32_t r[CW], u[CW];
+      tmem_ld_row(taddr + c * CW, r);
+      if (FX::kGated) tmem_ld_row(taddr + OW + c * CW, u);
+      uint32_t res_next[CW / 2];
+      if (has_res && c + 1 < c_end) load_residual<OutT>(fx, row, col0 + CW, p.M, p.N, res_vec_ok, res_next);
+      tc_wait_ld();
+      float v[CW];
+      fused_chunk<OWN>(r, u, rs, cs, (c - c_begin) * CW, same16, p, fx, v);
+      if (has_res) {
+        add_residual<OutT>(res, v);
+#pragma unroll
+        for (int j = 0; j < CW / 2; ++j) res[j] = res_next[j];
+      }
+      if (!MOE && p.out_tma) {
+        // 32 rows x CW columns leave as one TMA store, as in the plain epilogue: rows of 64 bytes in the 64-byte swizzle
+        // pattern, or of 32 bytes as they are
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < CW / 8; ++j)
+          *reinterpret_cast<uint4*>(out_stage + lane * (CW * 2) + (CW == 32 ? ((j ^ ((lane >> 1) & 3)) << 4) : (j << 4))) =
+              make_uint4(pack2<OutT>(v[8 * j], v[8 * j + 1]), pack2<OutT>(v[8 * j + 2], v[8 * j + 3]),
+                         pack2<OutT>(v[8 * j + 4], v[8 * j + 5]), pack2<OutT>(v[8 * j + 6], v[8 * j + 7]));
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && col0 < p.N && row < p.M) {  // (lane 0 has the block's first row)
+          tma_store_2d(&tmap_out, out_stage, col0, row);
+          tma_store_commit();
+        }
+      } else if (out_row >= 0 && col0 < p.N) {
+        store_values<OutT>(v, out_row, col0, p, vec_ok);
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tmem_empty_bar[buf]), 0));  // the accumulator is free again
+  }
+  if (lane == 0) tma_store_wait_all<0>();
+}
+
 // MOE: fused-MoE mode for blocks of 256 sorted slots (A8W8Params, "Fused-MoE mode"): a pair tile is one block, whose
 // expert picks the weight rows and column scales; the epilogue scatters each slot's row to its (token, choice) index.
-// EPI: epilogue warps per CTA, 4 or 8.  With 8 (the plain mode's default), two warps share a TMEM lane quarter and
+// EPI: epilogue warps per CTA, 4 or 8 (16 with a fused epilogue).  With 8 (the plain mode's default), two warps share a TMEM lane quarter and
 // split a tile's column chunks, and each has one output staging buffer instead of two.
 template <typename OutT, int BN, int STAGES, bool SK, bool MOE = false, int EPI = 4, class FX = NoEpilogue>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((2 + EPI) * 32, 1)
 a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                       const __grid_constant__ CUtensorMap tmap_out, const A8W8Params p, const FX fx) {
-  using L = PairSmem<BN, STAGES, EPI, FX::kOn>;
-  static_assert(EPI == 4 || (EPI == 8 && !SK && (!MOE || FX::kOn)), "eight epilogue warps exist for the plain mode only");
+  using L = PairSmem<BN, STAGES, EPI, FX>;
+  static_assert(EPI == 4 || (EPI == 8 && !SK && (!MOE || FX::kOn)) || (EPI == 16 && FX::kOn), "more than four epilogue warps exist for the plain mode and the fused epilogue only");
   static_assert(!(SK && FX::kOn), "no K-balanced mode with a fused epilogue");
   constexpr int OW = FX::kGated ? BN / 2 : BN;  // output columns of a tile
   static_assert(OW % 32 == 0, "whole chunks of 32 output columns");
@@ -832,40 +963,26 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         if (!mbar_wait_bounded(drain_bar, 0, &none)) report(p.status, abort_flag, DEV_TIMEOUT_DRAIN);
       }
     }
+  } else if constexpr (FX::kOn) {
+    pair_epilogue_fused<OutT, BN, L, MOE, EPI>(tmap_out, p, fx, smem, tmem_base, int(rank), pair_id, num_pairs, tmem_full_bar, tmem_empty_bar, abort_flag);
   } else {
     // -------------------------------- epilogue (both CTAs) --------------------------------
     const int quarter = warp & 3;
     const int ewarp = warp - 2;                  // 0 .. EPI-1
-    constexpr int NC = OW / 32;                  // column chunks of a tile
+    constexpr int NC = BN / 32;                  // column chunks of a tile
     const int c_begin = (EPI == 8 && ewarp >= 4) ? (NC + 1) / 2 : 0;  // with eight warps the second four take the upper chunks
     const int c_end = (EPI == 8 && ewarp < 4) ? (NC + 1) / 2 : NC;
-    float* cs = col_scale_smem + ewarp * L::kColWords;  // this warp's private copy
-    // (the expert products take the scales' product in fp32 whatever their dtypes are)
-    const bool same16 = !MOE && (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
+    float* cs = col_scale_smem + ewarp * BN;  // this warp's private copy
+    const bool same16 = (p.row_dtype == p.col_dtype) && (p.row_dtype != FNN_F32);
     const bool vec_ok = (p.ldo % 8 == 0) && (reinterpret_cast<uintptr_t>(p.out) % 16 == 0);
     const bool acc_vec_ok = p.acc_out && (p.ldacc % 4 == 0) && (reinterpret_cast<uintptr_t>(p.acc_out) % 16 == 0);
-    const int my_row = int(rank) * 128 + quarter * 32 + lane;           // this thread's row within a tile
-    bool res_vec_ok = false;
-    if constexpr (FX::kOn) res_vec_ok = (fx.ldr % 8 == 0) && (reinterpret_cast<uintptr_t>(fx.residual) % 16 == 0);
-    auto load_res = [&](int row, int col0, uint32_t (&r)[16]) { load_residual32<OutT>(fx, row, col0, p.M, p.N, res_vec_ok, r); };
-    // this thread's piece of the next tile's residual -> L2, a tile ahead
-    auto prefetch_res = [&](PairWork<SK, MOE> ahead) {
-      if constexpr (FX::kOn) {
-        if (!ahead.next()) return;
-        int mb, nb;
-        tile_coords(ahead.tile, p.tiles_m, p.tiles_n, mb, nb);
-        const int row = mb * 256 + my_row, col0 = nb * OW + c_begin * 32, col1 = min(nb * OW + c_end * 32, p.N);
-        if (row >= p.M) return;
-        const OutT* src = reinterpret_cast<const OutT*>(fx.residual) + int64_t(row) * fx.ldr;
-        for (int c = col0; c < col1; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
-      }
-    };
     int local = 0;
     bool ok = true;
     PairWork<SK, MOE> w(p, pair_id, num_pairs);
     uint8_t* out_stage = smem + L::kOutOff + ewarp * (L::kOutBufs * 2048);  // this warp's output staging buffer(s)
     int out_buf = 0;
     const int my_flag = int(rank) * 4 + quarter;                        // this warp's flag word within a pair's eight
+    const int my_row = int(rank) * 128 + quarter * 32 + lane;           // this thread's row within a tile
     for (; ok && w.next(); ++local) {
       int mb, nb;
       tile_coords(w.tile, p.tiles_m, p.tiles_n, mb, nb);
@@ -881,34 +998,21 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       const int last_h = adds ? ((w.tile + 1) * tail_blocks - 1) / p.sk_tail_units : -1;
       // slot of the piece of this tile that tail-sharing pair h computed: its pieces are of consecutive tiles
       auto slot_of = [&](int h) { return h * p.sk_slots + (w.tile - (h * p.sk_tail_units) / tail_blocks); };
-      const int n0 = nb * OW;
-      int64_t col_base = 0;
-      bool expert_ok = true;
-      if (MOE) {
-        const int e = __ldg(p.expert_ids + (mb * 256) / p.block_m);
-        if constexpr (FX::kOn) expert_ok = unsigned(e) < unsigned(fx.experts);
-        col_base = expert_ok ? int64_t(e) * p.col_stride_e : 0;
-      }
-      stage_columns<BN>(cs, c_begin * 32, (c_end - c_begin) * 32, n0, col_base, lane, p, fx);
-      if (FX::kGated) stage_columns<BN>(cs, OW + c_begin * 32, (c_end - c_begin) * 32, n0, col_base, lane, p, fx);
+      const int n0 = nb * BN;
+      const int64_t col_base = MOE ? int64_t(__ldg(p.expert_ids + (mb * 256) / p.block_m)) * p.col_stride_e : 0;
+      for (int j = c_begin * 32 + lane; j < c_end * 32; j += 32)
+        cs[j] = (n0 + j < p.N) ? load_as_f32(p.alpha_col, p.col_dtype, col_base + n0 + j) : 0.f;
       float rs = 0.f, rw = 1.f;
       int64_t out_row = -1;  // fused MoE: the flat (token, choice) index this slot writes, or -1
       if (MOE) {
         const int flat = __ldg(p.sorted_ids + row);
-        if (flat >= 0 && flat < p.num_valid && expert_ok) {
+        if (flat >= 0 && flat < p.num_valid) {
           out_row = flat;
           rs = load_as_f32(p.alpha_row, p.row_dtype, flat / p.top_k);
           if (p.mul_w) rw = load_as_f32(p.topk_w, p.topk_w_dtype, flat);
         }
       } else {
         rs = (row < p.M) ? load_as_f32(p.alpha_row, p.row_dtype, row) : 0.f;
-      }
-      uint32_t res[16];
-      if constexpr (FX::kOn) {
-        if (!MOE && fx.residual) {
-          load_res(row, n0 + c_begin * 32, res);
-          prefetch_res(w);
-        }
       }
       __syncwarp();
 
@@ -946,13 +1050,8 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       }
 #pragma unroll 1
       for (int c = c_begin; c < c_end; ++c) {
-        uint32_t r[32], u[32];
+        uint32_t r[32];
         tmem_ld_32x32(taddr + c * 32, r);
-        if (FX::kGated) tmem_ld_32x32(taddr + OW + c * 32, u);
-        uint32_t res_next[16];  // the residual is loaded a chunk ahead
-        if constexpr (FX::kOn) {
-          if (!MOE && fx.residual && c + 1 < c_end) load_res(row, n0 + (c + 1) * 32, res_next);
-        }
         uint4 cur[8];
         if (adds) {
 #pragma unroll
@@ -985,18 +1084,7 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             }
           }
         }
-        float v[32];
-        if constexpr (FX::kOn) {
-          fused_chunk<BN>(r, u, rs, cs, c * 32, same16, p, fx, v);
-          if (!MOE && fx.residual) {
-            add_residual32<OutT>(res, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) res[j] = res_next[j];
-          }
-        }
-        if (MOE && FX::kOn) {
-          if (out_row >= 0 && n0 + c * 32 < p.N) store_values<OutT>(v, out_row, n0 + c * 32, p, vec_ok);
-        } else if (MOE) {
+        if (MOE) {
           if (out_row >= 0) store_chunk_moe<OutT>(r, out_row, n0 + c * 32, rs, rw, p.mul_w != 0, cs + c * 32, p, vec_ok);
         } else if (p.out_tma) {
           // The 32 x 32 block of outputs goes through shared memory and leaves as one TMA store: whole 64-byte row
@@ -1004,10 +1092,9 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           // piece j of row l sits at piece j ^ ((l >> 1) & 3)), so the 32 lanes' stores spread over all banks; the
           // store leaves out what lies beyond M or N.  Two buffers per warp: before one is written again, the store
           // that read it two chunks ago has finished reading.
-          if (!FX::kOn) {
-            store_acc_chunk(r, row, n0 + c * 32, p, acc_vec_ok);
-            scale_chunk(r, rs, cs + c * 32, same16, p, v);
-          }
+          store_acc_chunk(r, row, n0 + c * 32, p, acc_vec_ok);
+          float v[32];
+          scale_chunk(r, rs, cs + c * 32, same16, p, v);
           if (lane == 0) tma_store_wait_read<L::kOutBufs - 1>();
           __syncwarp();
           uint8_t* buf_out = out_stage + out_buf * 2048;
@@ -1023,8 +1110,6 @@ a8w8_umma_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             tma_store_commit();
           }
           if (L::kOutBufs == 2) out_buf ^= 1;
-        } else if (FX::kOn) {
-          if (row < p.M && n0 + c * 32 < p.N) store_values<OutT>(v, row, n0 + c * 32, p, vec_ok);
         } else {
           store_chunk<OutT>(r, row, n0 + c * 32, rs, cs + c * 32, same16, p, vec_ok, acc_vec_ok);
         }
@@ -1173,7 +1258,7 @@ int launch_pair(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
   // for the operand ring; the output staging buffers and the column scales of the epilogue warps take the rest
   constexpr int kBudget = (EPI == 4 ? 196 : 194) * 1024;
   constexpr int STAGES = kBudget / (kBM * kBK + (BN / 2) * kBK) < 8 ? kBudget / (kBM * kBK + (BN / 2) * kBK) : 8;
-  using L = PairSmem<BN, STAGES, EPI, FX::kOn>;
+  using L = PairSmem<BN, STAGES, EPI, FX>;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
   static_assert(L::kStageBytes % 1024 == 0 && L::kABytes % 1024 == 0 && L::kOutOff % 1024 == 0, "tiles must stay 1024-byte aligned");
   static_assert(BN % 32 == 0 && BN <= 256, "pair tile width");
@@ -1195,7 +1280,7 @@ int launch_pair(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W8
   // output blocks of 32 rows x 32 columns (64 bytes per row) for the epilogue's TMA stores, where the output allows it
   p.out_tma = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && ((p.ldo * int64_t(sizeof(OutT))) % 16 == 0);
   if (p.out_tma) {
-    if (int e = make_tmap_2d(&tout, int(sizeof(OutT)), p.out, p.M, p.N, p.ldo * int64_t(sizeof(OutT)), 32, 32, /*swizzle=*/2)) return e;
+    if (int e = make_tmap_2d(&tout, int(sizeof(OutT)), p.out, p.M, p.N, p.ldo * int64_t(sizeof(OutT)), L::kChunk, 32, /*swizzle=*/L::kChunk == 32 ? 2 : 0)) return e;
   } else {
     tout = ta;  // never used
   }
@@ -1394,7 +1479,7 @@ int launch_moe_pair(const int8_t* a_sorted, int64_t EM, const int8_t* b, int64_t
   constexpr int OW = FX::kGated ? BN / 2 : BN;
   constexpr int kBudget = (EPI == 4 ? 196 : 194) * 1024;
   constexpr int STAGES = kBudget / (kBM * kBK + (BN / 2) * kBK);
-  using L = PairSmem<BN, STAGES, EPI, FX::kOn>;
+  using L = PairSmem<BN, STAGES, EPI, FX>;
   static_assert(L::kDynamicBytes <= 227 * 1024, "shared memory budget");
   auto kern = a8w8_umma_pair_kernel<OutT, BN, STAGES, false, true, EPI, FX>;
   static std::once_flag once[64];

@@ -84,42 +84,40 @@ __device__ __forceinline__ float activate_one(float v, int act) {
   return a[0];
 }
 
-// 32 consecutive residual values of one row as packed pairs; zeros outside the matrix
-template <typename T, class FX>
-__device__ __forceinline__ void load_residual32(const FX& fx, int row, int col0, int M, int N, bool vec_ok, uint32_t (&r)[16]) {
-  if constexpr (FX::kOn) {
-    if (row >= M || col0 >= N) {
+// 2 H consecutive residual values of one row as packed pairs; zeros outside the matrix
+template <typename T, int H, class FX>
+__device__ __forceinline__ void load_residual(const FX& fx, int row, int col0, int M, int N, bool vec_ok, uint32_t (&r)[H]) {
+  if (row >= M || col0 >= N) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = 0u;
-      return;
+    for (int j = 0; j < H; ++j) r[j] = 0u;
+    return;
+  }
+  const T* src = reinterpret_cast<const T*>(fx.residual) + int64_t(row) * fx.ldr + col0;
+  if (vec_ok && col0 + 2 * H <= N) {
+#pragma unroll
+    for (int j = 0; j < H; j += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + 2 * j);
+      r[j] = u.x; r[j + 1] = u.y; r[j + 2] = u.z; r[j + 3] = u.w;
     }
-    const T* src = reinterpret_cast<const T*>(fx.residual) + int64_t(row) * fx.ldr + col0;
-    if (vec_ok && col0 + 32 <= N) {
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 u = *reinterpret_cast<const uint4*>(src + 8 * j);
-        r[4 * j] = u.x; r[4 * j + 1] = u.y; r[4 * j + 2] = u.z; r[4 * j + 3] = u.w;
-      }
-    } else {
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const uint32_t lo = col0 + 2 * j < N ? h[2 * j] : 0u, hi = col0 + 2 * j + 1 < N ? h[2 * j + 1] : 0u;
-        r[j] = lo | (hi << 16);
-      }
+    for (int j = 0; j < H; ++j) {
+      const uint32_t lo = col0 + 2 * j < N ? h[2 * j] : 0u, hi = col0 + 2 * j + 1 < N ? h[2 * j + 1] : 0u;
+      r[j] = lo | (hi << 16);
     }
   }
 }
-template <typename T> __device__ __forceinline__ void add_residual32(const uint32_t (&r)[16], float (&v)[32]) {
+template <typename T, int H> __device__ __forceinline__ void add_residual(const uint32_t (&r)[H], float (&v)[2 * H]) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < H; ++j) {
     v[2 * j] = __fadd_rn(v[2 * j], lo_of<T>(r[j]));
     v[2 * j + 1] = __fadd_rn(v[2 * j + 1], hi_of<T>(r[j]));
   }
 }
-__device__ __forceinline__ void add_bias32(const float* b, float (&v)[32]) {
+template <int N> __device__ __forceinline__ void add_bias(const float* b, float (&v)[N]) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     const float4 t = *reinterpret_cast<const float4*>(b + j);
     v[j] = __fadd_rn(v[j], t.x); v[j + 1] = __fadd_rn(v[j + 1], t.y);
     v[j + 2] = __fadd_rn(v[j + 2], t.z); v[j + 3] = __fadd_rn(v[j + 3], t.w);

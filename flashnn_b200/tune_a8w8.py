@@ -4,7 +4,7 @@ flashnn/triton_kernels/triton_utils.py:84-151).
     python -m flashnn_b200.tune_a8w8 --measure > points.jsonl     # on a B200: times every pair-tile width per shape
     python -m flashnn_b200.tune_a8w8 --fit points.jsonl           # anywhere: writes csrc/a8w8_plan.h
 
-The planner in csrc/gemm_a8w8.cu predicts the time of a launch as waves x tile width x a per-width cost of one
+The planner in csrc/a8w8_kernels.cuh predicts the time of a launch as waves x tile width x a per-width cost of one
 output column (narrow tiles re-read the A rows for fewer columns).  `--fit` derives those per-width costs from the
 measured points: for every shape, time(width) / time(256) divided by the same ratio of waves x width, then the
 median over shapes.  The header it writes holds the constants and, as a comment, the measured table they came from.

@@ -86,18 +86,20 @@ def test_every_activation_on_every_kernel(act, gated, m):
         check_gemm(c, act, gated, out_ty)
 
 
-def test_every_width_of_the_pair_tile_is_reached():
+@pytest.mark.parametrize("k", [128, 2304])  # with 16 and with 8 epilogue warps
+def test_every_width_of_the_pair_tile_is_reached(k):
     """The shape table's widths for the plain product decide the fused one's too; each of them runs here."""
     from flashnn_b200 import _lib
     seen = set()
     for m, n in [(4096, 8192), (4096, 7168), (764, 8192), (2048, 4736), (1024, 4700), (1024, 4400), (512, 4736), (300, 9400)]:
-        kernel, width = _lib.a8w8_plan(m, n, 128)
+        kernel, width = _lib.a8w8_plan(m, n, k)
         if kernel == 1 and width not in seen:
             seen.add(width)
-            check_gemm(gemm_case(m, n, 128, False, True, True, torch.bfloat16, seed=width), "silu", False, torch.bfloat16)
+            check_gemm(gemm_case(m, n, k, False, True, True, torch.bfloat16, seed=width), "silu", False, torch.bfloat16)
     assert len(seen) >= 3
     for m, n in [(4096, 4096), (764, 4096), (512, 2368), (1024, 2200)]:
-        check_gemm(gemm_case(m, n, 128, True, True, True, torch.bfloat16, seed=n), "silu", True, torch.bfloat16)
+        check_gemm(gemm_case(m, n, k, True, True, True, torch.bfloat16, seed=n), "silu", True, torch.bfloat16)
+    check_gemm(gemm_case(700, 4999, k, False, False, True, torch.float16, seed=k), "gelu", False, torch.float16)  # an output that takes no TMA stores
 
 
 @pytest.mark.parametrize("m", [4, 40, 400])
@@ -171,7 +173,8 @@ def _call_c(c, act, gated, out, ldo, residual, ldr):
 
 
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("m,n,k,ldo", [(3, 520, 4096, 528), (70, 100, 144, 107), (70, 96, 144, 104), (300, 1000, 144, 1008), (300, 333, 144, 334)])
+@pytest.mark.parametrize("m,n,k,ldo", [(3, 520, 4096, 528), (70, 100, 144, 107), (70, 96, 144, 104), (300, 1000, 144, 1008), (300, 333, 144, 334), (16, 200, 4096, 203),
+                                       (700, 5000, 2304, 5008)])
 def test_writes_stay_inside_and_the_residual_may_be_the_output(m, n, k, ldo, gated):
     c = gemm_case(m, n, k, gated, True, True, torch.bfloat16, seed=ldo)
     value, bound = O.gemm_epilogue(c["a"], c["b"], c["row"], c["col"], c["bias"], "silu", gated, c["residual"], torch.bfloat16)
@@ -300,6 +303,25 @@ def test_routing_masked_and_non_finite_rows():
     assert (ids.sort(1).values == torch.arange(24, device="cuda")).all()
 
 
+@pytest.mark.parametrize("e,k", [(40, 12), (200, 6)])
+def test_many_rows_that_fp32_does_not_decide(e, k):
+    """The same doubtful row 50000 times: every copy is decided alike, in 64 bits, by both forms of the kernel."""
+    import flashnn_b200
+    g = _gen(e)
+    x = torch.randn(1, e, generator=g, device="cuda").abs() * 2 ** -20
+    bias = torch.rand(e, generator=g, device="cuda") * 2 ** -20
+    w, ids = check_route(x, k, bias, scoring="sigmoid")
+    many = flashnn_b200.MoeRouting(e, k, scoring="sigmoid")(x.expand(50000, -1), bias)
+    assert (many[0] == w).all() and (many[1] == ids).all()
+
+
+def test_equal_logits_choose_the_first_experts():
+    import flashnn_b200
+    for e, k in ((8, 2), (256, 8), (64, 6), (1000, 20)):  # a router that has learnt nothing yet
+        w, ids = flashnn_b200.MoeRouting(e, k)(torch.zeros(300, e, device="cuda", dtype=torch.bfloat16))
+        assert (ids == torch.arange(k, device="cuda")).all() and torch.allclose(w, torch.full_like(w, 1 / k), rtol=1e-6)
+
+
 def test_routing_strided_logits_and_empty_batch():
     import flashnn_b200
     f = flashnn_b200.MoeRouting(40, 4)
@@ -317,7 +339,7 @@ def test_routing_strided_logits_and_empty_batch():
 # expert sort
 # ---------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("n,e,bm", [(1, 1, 1), (1, 8, 16), (2, 8, 16), (31, 3, 16), (1000, 60, 32), (4096, 8, 128), (4097, 256, 64),
-                                    (20001, 512, 256), (131072, 256, 128), (70000, 1024, 16), (50000, 7, 100)])
+                                    (20001, 512, 256), (131072, 256, 128), (70000, 1024, 16), (50000, 7, 100), (300000, 100, 64)])
 def test_expert_sort(n, e, bm):
     import flashnn_b200
     g = _gen(n)

@@ -38,6 +38,8 @@ struct RouteParams {
   float scale;
   int wide;        // lanes read whole words (set by the launch)
   int whole_lanes; // a group is a power of two of lanes with all of their experts (set by the launch)
+  int used;        // experts of a lane in the kernel with several tokens per warp, and whether its 64-bit form reads whole words
+  int wide_64;
 };
 
 // maxima and minima that skip a NaN, which marks what is not there
@@ -138,9 +140,9 @@ template <typename T> __device__ __forceinline__ void load_word(const T* src, bo
   }
 }
 template <typename T, int PER>
-__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, float (&x)[PER]) {
+__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t row, int lane, bool wide, float (&x)[PER]) {
   const T* src = reinterpret_cast<const T*>(p.logits) + row * p.ldl + lane * PER;
-  if (PER >= 4 && p.wide) {
+  if (PER >= 4 && wide) {
     const bool on = lane * PER < p.E;
 #pragma unroll
     for (int w = 0; w < PER; w += 4) {
@@ -352,7 +354,7 @@ __device__ __forceinline__ bool route_row(const RouteParams& p, const float (&x)
 template <typename T, int PER>
 __device__ __noinline__ void route_row_64(const RouteParams& p, int64_t row, int lane, const float* s_bias, double* s_keys) {
   float x[PER];
-  load_logits<T, PER>(p, row, lane, x);
+  load_logits<T, PER>(p, row, lane, p.wide_64 != 0, x);
   route_row<double, T, PER>(p, x, row, lane, s_bias, s_keys);
 }
 
@@ -375,11 +377,11 @@ __global__ void __launch_bounds__(WARPS * 32, 24 / WARPS) moe_route_kernel(const
   while (row < p.M) {
     int put_off = 0;
     float x[PER];
-    load_logits<T, PER>(p, row, lane, x);
+    load_logits<T, PER>(p, row, lane, p.wide != 0, x);
     while (true) {
       const int64_t next = row + step;
       float ahead[PER];
-      if (next < p.M) load_logits<T, PER>(p, next, lane, ahead);
+      if (next < p.M) load_logits<T, PER>(p, next, lane, p.wide != 0, ahead);
       if (!route_row<float, T, PER>(p, x, row, lane, s_bias, reinterpret_cast<float*>(s_keys[warp]))) s_put_off[warp][put_off++] = row;
       row = next;
       if (row >= p.M || put_off == kPutOff) break;
@@ -392,9 +394,9 @@ __global__ void __launch_bounds__(WARPS * 32, 24 / WARPS) moe_route_kernel(const
   }
 }
 
-// The usual shapes: top_k <= 8.  W lanes per token (several tokens per warp), lane s of them with experts s * PER .. s * PER + PER - 1 in
-// registers.  What the one-warp kernel spends on its rounds (37 instructions each) goes into networks of minima and maxima that
-// need no expert numbers: a lane sorts its keys eight at a time and merges them into its eight largest, a butterfly merges the lanes',
+// The usual shapes: top_k <= 16.  W lanes per token (several tokens per warp), lane s of them with experts s * used .. s * used + used - 1, used <= PER, in
+// registers, so that a group is whole lanes.  What the one-warp kernel spends on its rounds (37 instructions each) goes into networks of minima and maxima that
+// need no expert numbers: a lane sorts its keys eight (or 16) at a time and merges them into its eight largest, a butterfly merges the lanes',
 // and the top_k-th of the result is all that is kept.  The keys that are not below it, less the tolerance, are the candidates,
 // top_k of them and rarely more; in a list, in expert order, each counts those before it, and that is its place.
 // 16384 tokens x 256 experts in groups, fp32 logits: one warp per token 980 instructions a row and 28 us, this kernel 430 and 17 us.
@@ -407,39 +409,43 @@ template <typename F, int N> __device__ __forceinline__ void merge_largest(F (&a
   merge_bitonic<N / 2>(a);
 }
 
-constexpr int kListCap = 16;
-
-template <typename T, int PER, int W, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel(const __grid_constant__ RouteParams p) {
+// LIST: largest keys that a lane keeps, 8 or 16, at least top_k; the list of candidates holds twice as many.
+template <typename T, int PER, int W, int LIST, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (LIST == 8 ? 28 : 20) / WARPS) moe_route_lists_kernel(const __grid_constant__ RouteParams p) {
+  static_assert(LIST <= W, "a lane for every choice");
   constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kListCap = 2 * LIST;
   constexpr int kRows = 32 / W;  // tokens a warp works on
   __shared__ double s_keys[WARPS][W * PER <= 256 ? 256 : W * PER];  // for the rows that were put off (one warp per row: 32 lanes)
-  __shared__ float4 s_bias4[W * PER / 4];
+  __shared__ float4 s_bias4[W * PER / 4], s_lane_bias4[W * PER / 4];  // by expert, and by lane (PER words each)
   __shared__ alignas(16) float s_key[WARPS][kRows][kListCap];
   __shared__ float s_x[WARPS][kRows][kListCap];
   __shared__ int s_id[WARPS][kRows][kListCap];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % W, mine = lane / W;
-  float* s_bias = reinterpret_cast<float*>(s_bias4);
+  float *s_bias = reinterpret_cast<float*>(s_bias4), *s_lane_bias = reinterpret_cast<float*>(s_lane_bias4);
   if (p.bias) {
-    for (int e = threadIdx.x; e < W * PER; e += WARPS * 32) s_bias[e] = e < p.E ? __ldg(p.bias + e) : 0.f;
+    for (int i = threadIdx.x; i < W * PER; i += WARPS * 32) {
+      const int e = i / PER * p.used + i % PER;
+      s_bias[i] = i < p.E ? __ldg(p.bias + i) : 0.f;
+      s_lane_bias[i] = i % PER < p.used && e < p.E ? __ldg(p.bias + e) : 0.f;
+    }
     __syncthreads();
   }
   const float inf = __int_as_float(0x7f800000);
   const int64_t row = (int64_t(blockIdx.x) * WARPS + warp) * kRows + mine;
   const bool live = row < p.M;
-  const int e0 = sub * PER;
+  const int e0 = sub * p.used;
   const bool by_logit = p.bias == nullptr && !p.summed;
-  const int present = min(max(p.E - e0, 0), PER);
+  const int present = min(max(p.E - e0, 0), p.used);
 
   float key[PER];
   const T* src = reinterpret_cast<const T*>(p.logits) + (live ? row : 0) * p.ldl;
   {
-    const bool on = present > 0;
     if (p.wide) {
 #pragma unroll
       for (int w = 0; w < PER; w += 4) {
         float v[4];
-        load_word(src + e0 + w, on, v);
+        load_word(src + e0 + w, w < present, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) key[w + j] = v[j];
       }
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel
     if (p.bias) {
 #pragma unroll
       for (int j = 0; j < PER; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(s_bias + e0 + j);
+        const float4 b = *reinterpret_cast<const float4*>(s_lane_bias + sub * PER + j);
         key[j] += b.x; key[j + 1] += b.y; key[j + 2] += b.z; key[j + 3] += b.w;
       }
     }
@@ -521,7 +527,7 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel
 
   if (p.groups > 1) {
     // (groups are whole lanes, a power of two of them: checked on the host)
-    const int lanes = p.group_size / PER, g = sub / lanes;
+    const int lanes = p.group_size / p.used, g = sub / lanes;
     const bool two = p.summed && p.group_size > 1;
     float a = -inf, b = -inf;
 #pragma unroll
@@ -579,34 +585,36 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel
   }
 
   // the top_k-th largest key
-  float best[8];
-  if constexpr (PER >= 8) {
+  constexpr int kRun = PER < LIST ? PER : LIST;  // keys sorted at a time
+  float best[LIST];
+  {
+    float run[kRun];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) best[j] = key[j];
-    sort_descending(best);
+    for (int j = 0; j < kRun; ++j) run[j] = key[j];
+    sort_descending(run);
 #pragma unroll
-    for (int c = 8; c < PER; c += 8) {
-      float more[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) more[j] = key[c + j];
-      sort_descending(more);
-      merge_largest(best, more);
-    }
+    for (int j = 0; j < LIST; ++j) best[j] = j < kRun && in ? run[j < kRun ? j : 0] : -inf;
   }
-  if (!in) {
+  if constexpr (PER > LIST) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) best[j] = -inf;
+    for (int c = LIST; c < PER; c += LIST) {
+      float run[LIST];
+#pragma unroll
+      for (int j = 0; j < LIST; ++j) run[j] = in ? key[c + j] : -inf;
+      sort_descending(run);
+      merge_largest(best, run);
+    }
   }
 #pragma unroll
   for (int o = 1; o < W; o <<= 1) {
-    float other[8];
+    float other[LIST];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) other[j] = __shfl_xor_sync(kAll, best[j], o);
+    for (int j = 0; j < LIST; ++j) other[j] = __shfl_xor_sync(kAll, best[j], o);
     merge_largest(best, other);
   }
   float least = best[0];
 #pragma unroll
-  for (int j = 1; j < 8; ++j) least = j < p.top_k ? best[j] : least;
+  for (int j = 1; j < LIST; ++j) least = j < p.top_k ? best[j] : least;
   if (check) least -= 2.1f * (off + rel * fabsf(least));
   bool odd = !(least > -inf);  // fewer keys than choices above -infinity: the general form knows what is there
 
@@ -637,25 +645,25 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel
     }
   }
   __syncwarp();
-  // every lane counts those before its candidates sub and sub + 8; then lane s holds choice s
+  // every lane counts those before its candidates sub and sub + LIST; then lane s holds choice s
   const int listed = odd ? 0 : count;
   float cx[2], ck[2];
   int place[2], cid[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const int t = sub + 8 * c;
-    const bool on = sub < 8 && t < listed;
+    const int t = sub + LIST * c;
+    const bool on = sub < LIST && t < listed;
     ck[c] = on ? s_key[warp][mine][t] : 0.f;
     cx[c] = on ? s_x[warp][mine][t] : 0.f;
     cid[c] = on ? s_id[warp][mine][t] : 0;
     place[c] = on ? 0 : kListCap;
   }
-  const bool more = __any_sync(kAll, listed > 8);
+  const bool more = __any_sync(kAll, listed > LIST);
 #pragma unroll 2
-  for (int t = 0; t < (more ? kListCap : 8); ++t) {
+  for (int t = 0; t < (more ? kListCap : LIST); ++t) {
     const float other = t < listed ? s_key[warp][mine][t] : -inf;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) place[c] += (other > ck[c] || (other == ck[c] && t < sub + 8 * c && t < listed)) ? 1 : 0;
+    for (int c = 0; c < 2; ++c) place[c] += (other > ck[c] || (other == ck[c] && t < sub + LIST * c && t < listed)) ? 1 : 0;
   }
   bool chosen = false;
   float k = 0.f, x = 0.f;
@@ -688,14 +696,14 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel
         if (!more) break;
       }
       if (!more) k64[1] = 0.0;
-      place[0] = sub < 8 && sub < listed ? 0 : kListCap;
-      place[1] = sub < 8 && sub + 8 < listed ? 0 : kListCap;
+      place[0] = sub < LIST && sub < listed ? 0 : kListCap;
+      place[1] = sub < LIST && sub + LIST < listed ? 0 : kListCap;
 #pragma unroll 1
       for (int t = 0; t < kListCap; ++t) {
-        const double other = __shfl_sync(kAll, t < 8 ? k64[0] : k64[1], mine * W + (t & 7));
+        const double other = __shfl_sync(kAll, t < LIST ? k64[0] : k64[1], mine * W + t % LIST);
         if (t < listed) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) place[c] += (other > k64[c] || (other == k64[c] && t < sub + 8 * c)) ? 1 : 0;
+          for (int c = 0; c < 2; ++c) place[c] += (other > k64[c] || (other == k64[c] && t < sub + LIST * c)) ? 1 : 0;
         }
       }
       in_order();
@@ -730,20 +738,27 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) moe_route_lists_kernel
   }
 }
 
-template <typename T, int PER, int W>
-int launch_route_lists(RouteParams p, cudaStream_t st) {
+// Experts of a lane (at most per), so that a group is a power of two of whole lanes and all fit in w of them; 0 if there is no such number.
+inline int lane_experts(const RouteParams& p, int per, int w) {
+  if (p.groups == 1) return p.E <= per * w ? per : 0;
+  for (int lanes = 1; p.groups * lanes <= w; lanes *= 2)
+    if (p.group_size % lanes == 0 && p.group_size / lanes <= per) return p.group_size / lanes;
+  return 0;
+}
+
+template <typename T, int PER, int W, int LIST>
+bool launch_route_lists(RouteParams p, cudaStream_t st, int& status) {
   constexpr int kWarps = 4, kPer64 = (W * PER + 31) / 32;
   const int64_t rows = kWarps * (32 / W);
-  p.wide = p.E % PER == 0 && reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && (p.ldl * int64_t(sizeof(T))) % 16 == 0;
+  p.used = lane_experts(p, PER, W);
+  if (p.used == 0) return false;
+  p.wide = p.E % 4 == 0 && p.used % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && (p.ldl * int64_t(sizeof(T))) % 16 == 0;
   const int lanes = p.group_size / kPer64;  // (of the 64-bit form)
   p.whole_lanes = p.group_size % kPer64 == 0 && (lanes & (lanes - 1)) == 0;
-  moe_route_lists_kernel<T, PER, W, kWarps><<<unsigned((p.M + rows - 1) / rows), kWarps * 32, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "moe_route launch");
-}
-// whether a group is a power of two of lanes with PER experts each
-inline bool whole_lanes(const RouteParams& p, int per) {
-  const int lanes = p.group_size / per;
-  return p.groups == 1 || (p.group_size % per == 0 && (lanes & (lanes - 1)) == 0);
+  p.wide_64 = p.wide && p.E % kPer64 == 0;
+  moe_route_lists_kernel<T, PER, W, LIST, kWarps><<<unsigned((p.M + rows - 1) / rows), kWarps * 32, 0, st>>>(p);
+  status = check_cuda(cudaGetLastError(), "moe_route launch");
+  return true;
 }
 
 template <typename T, int PER>
@@ -753,6 +768,7 @@ int launch_route_per(RouteParams p, cudaStream_t st) {
   const bool full = p.E % PER == 0;
   const int word = PER * int(sizeof(T)) < 16 ? PER * int(sizeof(T)) : 16;
   p.wide = full && reinterpret_cast<uintptr_t>(p.logits) % word == 0 && (p.ldl * int64_t(sizeof(T))) % word == 0;
+  p.wide_64 = p.wide;
   const int lanes = p.group_size / PER;
   p.whole_lanes = p.group_size % PER == 0 && (lanes & (lanes - 1)) == 0;
   const int64_t blocks = (int64_t(p.M) + kWarps - 1) / kWarps, resident = int64_t(sm_count()) * (24 / kWarps);
@@ -762,12 +778,15 @@ int launch_route_per(RouteParams p, cudaStream_t st) {
 
 template <typename T>
 int launch_route(const RouteParams& p, cudaStream_t st) {
-  if (p.top_k <= 8 && p.E > 32) {
-    if (p.E <= 64 && whole_lanes(p, 8)) return launch_route_lists<T, 8, 8>(p, st);
-    if (p.E > 64 && p.E <= 128 && whole_lanes(p, 16)) return launch_route_lists<T, 16, 8>(p, st);
-    if (p.E > 128 && p.E <= 256 && whole_lanes(p, 32)) return launch_route_lists<T, 32, 8>(p, st);
-    if (p.E > 256 && p.E <= 512 && whole_lanes(p, 32)) return launch_route_lists<T, 32, 16>(p, st);
-  }
+  int status = FNN_OK;
+  if (p.E > 32 && p.top_k <= 8 &&
+      (launch_route_lists<T, 8, 8, 8>(p, st, status) || launch_route_lists<T, 16, 8, 8>(p, st, status) ||
+       launch_route_lists<T, 32, 8, 8>(p, st, status) || launch_route_lists<T, 32, 16, 8>(p, st, status)))
+    return status;
+  if (p.E > 32 && p.top_k > 8 && p.top_k <= 16 &&
+      (launch_route_lists<T, 8, 16, 16>(p, st, status) || launch_route_lists<T, 16, 16, 16>(p, st, status) ||
+       launch_route_lists<T, 32, 16, 16>(p, st, status)))
+    return status;
   const int per = (p.E + 31) / 32;
   if (per <= 1) return launch_route_per<T, 1>(p, st);
   if (per <= 2) return launch_route_per<T, 2>(p, st);

@@ -233,7 +233,8 @@ def check_route(logits, top_k, bias=None, **kw):
 
 
 ROUTES = [(1, 1, 1, 1, 1), (1, 8, 2, 1, 1), (7, 5, 5, 1, 1), (64, 60, 4, 1, 1), (33, 64, 6, 8, 3), (50, 160, 6, 8, 3), (129, 256, 8, 8, 4),
-          (20, 384, 8, 1, 1), (9, 1000, 32, 1, 1), (16, 1024, 16, 32, 5), (40, 72, 3, 12, 4), (30, 32, 32, 32, 32), (11, 96, 7, 3, 2)]
+          (20, 384, 8, 1, 1), (9, 1000, 32, 1, 1), (16, 1024, 16, 32, 5), (40, 72, 3, 12, 4), (30, 32, 32, 32, 32), (11, 96, 7, 3, 2),
+          (50, 448, 15, 8, 5), (21, 60, 5, 4, 3), (17, 510, 8, 3, 2), (40, 120, 12, 8, 4), (13, 250, 9, 2, 1), (35, 36, 16, 1, 1)]
 
 
 @pytest.mark.parametrize("shape", ROUTES, ids=str)

@@ -607,6 +607,89 @@ def test_a_layer_in_two_captured_graphs_and_on_two_streams():
             within(out, *O.combine(h, w))
 
 
+def test_the_product_captured_and_replayed_on_new_inputs():
+    """Each kernel of the product in one graph (streaming, cluster, single CTA, CTA pair), replayed twice beside eager calls."""
+    import flashnn_b200 as F
+    shapes = [(2, 512, 4096), (16, 200, 4096), (100, 2000, 256), (400, 1000, 512)]
+    f = F.GemmA8W8Epilogue(torch.bfloat16, "silu", gated=True)
+
+    def call(c):
+        return f(c["a"], c["b"], c["row"], c["col"], bias=c["bias"], residual=c["residual"])
+    cases = [[gemm_case(*s, True, True, True, torch.bfloat16, seed=i) for s in shapes] for i in range(3)]
+    want = [[call(c) for c in row] for row in cases]
+    static = cases[0]
+    static = [{k: v.clone() for k, v in c.items()} for c in static]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        outs = [call(c) for c in static]
+    for i in (1, 2):
+        for c, new in zip(static, cases[i]):
+            for k in c:
+                c[k].copy_(new[k])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            g.replay()
+        eager = [call(c) for c in cases[0]]  # on the default stream, at the same time
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[i])) and all(torch.equal(a, b) for a, b in zip(eager, want[0]))
+
+
+def test_an_expert_chosen_twice_by_one_token():
+    c = experts_case(20, 4, 64, 96, 3, True, torch.bfloat16, seed=6)
+    c["ids"][:, 2] = c["ids"][:, 0]
+    out = check_experts(c, "silu", 16, torch.bfloat16)
+    assert torch.equal(out[:, 2], out[:, 0])
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# offsets that pass 32 bits
+# ---------------------------------------------------------------------------------------------------------------
+def test_outputs_and_residual_beyond_32_bit_offsets():
+    m, n, k = 36000, 60000, 64  # 2.16e9 outputs
+    c = gemm_case(m, n, k, False, True, False, torch.bfloat16, seed=1)
+    c["residual"] = torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")
+    rows = torch.tensor([0, 17, m // 2, m - 1], device="cuda")
+    c["residual"][rows] = torch.randn(4, n, device="cuda").bfloat16()
+    out = run_gemm(c, "relu", False, torch.bfloat16)
+    within(out[rows], *O.gemm_epilogue(c["a"][rows], c["b"], c["row"][rows], c["col"], c["bias"], "relu", False, c["residual"][rows], torch.bfloat16))
+
+
+def test_expert_weights_and_outputs_beyond_32_bit_offsets():
+    import flashnn_b200 as F
+    e, n, k, top_k = 40, 14336, 4096, 2  # 4.7e9 bytes of weights
+    g = _gen(0)
+    b = torch.randint(-127, 128, (e, 2 * n, k), generator=g, device="cuda", dtype=torch.int8)
+    ids = torch.tensor([[39, 0], [1, 38], [39, 37]], device="cuda", dtype=torch.int32)
+    c = dict(a=torch.randint(-127, 128, (3, k), generator=g, device="cuda", dtype=torch.int8), b=b, row=torch.full((3,), 0.01, device="cuda"),
+             col=torch.full((e, 2 * n), 1 / (0.01 * 5376 * 64), device="cuda"), bias=None, ids=ids)
+    check_experts(c, "silu", 16, torch.bfloat16)
+    # 2.2e9 outputs: 80000 tokens, few of them checked
+    m, n = 80000, 14000
+    c = experts_case(m, 3, n, 64, 2, False, torch.float16, seed=3)
+    out = torch.empty(m, 2, n, dtype=torch.float16, device="cuda")
+    plan = F.moe_sort_tokens(c["ids"], 3, 256)
+    F.fused_moe_a8w8_gated_forward(c["a"], c["b"], out, c["row"], c["col"], c["ids"], *plan, 2, 256)
+    rows = torch.tensor([0, 5, m // 2, m - 1], device="cuda")
+    within(out[rows], *O.experts_gated(c["a"][rows], c["b"], c["row"][rows], c["col"], None, "silu", c["ids"][rows], torch.float16))
+    del out, plan, b
+    torch.cuda.empty_cache()
+
+
+def test_logits_beyond_32_bit_offsets():
+    m, e = 2 ** 23 + 37, 256
+    x = torch.randn(m, e, device="cuda", dtype=torch.bfloat16)
+    import flashnn_b200 as F
+    w, ids = F.MoeRouting(e, 4)(x)
+    rows = torch.tensor([0, 1, m // 2, m - 2, m - 1], device="cuda")
+    rw, rids = O.route(x[rows].cpu(), 4)
+    assert torch.equal(ids[rows].cpu(), rids)
+    within(w[rows].cpu(), rw, rw.abs() * 4e-5)
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_calls_on_a_stream_that_is_not_the_default():
     x = layer_case(64, seed=5)
     want = moe_layer(*x, top_k=2, bm=16)[0]

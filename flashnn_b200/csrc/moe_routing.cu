@@ -1069,35 +1069,46 @@ extern "C" int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_
   if (!num_tokens_post_padded || (num_choices > 0 && (!topk_ids || !sorted_token_ids || !expert_ids)))
     return fail(FNN_ERR_NULL_POINTER, "moe_sort: null tensor pointer");
   SortParams p{topk_ids, sorted_token_ids, expert_ids, num_tokens_post_padded, int(num_choices), int(E), block_m, int(first_expert), int(EM)};
+  // 16 CTAs are more than every device promises a cluster (a partition may not hold them): asked once for the largest launch
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
+  static unsigned most_ctas[64];
   int dev = 0;
   cudaGetDevice(&dev);
   dev &= 63;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   std::call_once(once[dev], [&] {
-    attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortWarps + 4) * kSortMaxExperts * 4);
+    constexpr int kMostBytes = (kSortWarps + 4) * kSortMaxExperts * 4;
+    attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes);
     if (attr_err[dev] == cudaSuccess) attr_err[dev] = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = kMostBytes;
+    attr[0].val.clusterDim.x = 16;
+    int clusters = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, moe_sort_kernel, &cfg);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    most_ctas[dev] = e == cudaSuccess && clusters > 0 ? 16u : 8u;
   });
   if (attr_err[dev] != cudaSuccess) return check_cuda(attr_err[dev], "cudaFuncSetAttribute(moe_sort)");
-  cudaLaunchConfig_t cfg = {};
   // One CTA where a launch is all there is to it, else as many as a cluster holds: they write the slots, padding included, and 16 SMs
   // write them faster than one.  Measured, one CTA / a cluster: 64 tokens x 2 of 8 experts (240 slots) 4.4 / 5.4 us, 512 x 2 of 8
   // in blocks of 128 (1920) 5.3 / 5.6, 2048 x 2 of 8 (4992) 7.9 / 5.8, 64 x 8 of 256 (32768) 18 / 6.7.  A cluster of 8: 131072
   // choices 16.8 us, of 16: 12.1.  Warps cost barriers, and pay where their steps (32 choices each) are many: 512 / 1024
   // threads a CTA, 16384 choices 7.4 / 8.7 us, 131072 12.1 / 12.7, 262144 22.9 / 17.8.
-  const unsigned ctas = need > 2048 ? 16u : 1u;
+  const unsigned ctas = need > 2048 ? most_ctas[dev] : 1u;
   unsigned threads = ctas == 1 ? 256u : num_choices > 131072 ? unsigned(kSortThreads) : 512u;
   if (int64_t(threads) < E) threads = unsigned((E + 31) / 32 * 32);
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = size_t(threads / 32 + 4) * size_t(E) * sizeof(int32_t);
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, moe_sort_kernel, p), "moe_sort launch");
 }
 

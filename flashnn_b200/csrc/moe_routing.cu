@@ -956,65 +956,96 @@ struct CombineParams {
   int M, N, top_k, E, first;
 };
 
-// VEC: columns of a thread, 8 (16-byte accesses) or 1
-template <typename T, int VEC>
+// VEC: columns of an access, 8, 2 or 1, as N and the alignments allow; GROUPS: accesses of a thread and row, 256 * VEC
+// columns apart, so that narrow accesses have as many bytes in flight.
+template <typename T, int VEC> struct CombineWord { using type = T; };
+template <typename T> struct CombineWord<T, 8> { using type = uint4; };
+template <typename T> struct CombineWord<T, 2> { using type = uint32_t; };
+
+template <typename T, int VEC, int GROUPS>
 __global__ void __launch_bounds__(256) moe_combine_kernel(const CombineParams p) {
   const int64_t m = blockIdx.x;
-  const int n = (blockIdx.y * 256 + threadIdx.x) * VEC;
+  const int n = blockIdx.y * (256 * GROUPS * VEC) + threadIdx.x * VEC;
   if (n >= p.N) return;
-  float acc[VEC];
+  float acc[GROUPS][VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  using Word = typename std::conditional<VEC == 8, uint4, T>::type;
-  auto add = [&](const Word& v, float w) {
+  for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[g][j] = 0.f;
+  using Word = typename CombineWord<T, VEC>::type;
+  auto add = [&](int g, const Word& v, float w) {
     if constexpr (VEC == 8) {
       const uint32_t a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        acc[2 * j] = fmaf(w, lo_of<T>(a[j]), acc[2 * j]);
-        acc[2 * j + 1] = fmaf(w, hi_of<T>(a[j]), acc[2 * j + 1]);
+        acc[g][2 * j] = fmaf(w, lo_of<T>(a[j]), acc[g][2 * j]);
+        acc[g][2 * j + 1] = fmaf(w, hi_of<T>(a[j]), acc[g][2 * j + 1]);
       }
+    } else if constexpr (VEC == 2) {
+      acc[g][0] = fmaf(w, lo_of<T>(v), acc[g][0]);
+      acc[g][1] = fmaf(w, hi_of<T>(v), acc[g][1]);
     } else {
-      acc[0] = fmaf(w, to_f32(v), acc[0]);
+      acc[g][0] = fmaf(w, to_f32(v), acc[g][0]);
     }
   };
+  auto there = [&](int g) { return n + g * 256 * VEC < p.N; };
   // Two choices' rows at a time, their loads in flight together; a choice that is not here is neither read nor added.  One at a time
   // / two / four / eight: 4096 tokens x 8 choices (an eighth of them gone) x 4096 55 / 50 / 52 / 61 us, 16384 x 2 x 4096 93 / 86 / 114 / 182.  The reads
   // bound it: 50 us are 6.7 TB/s.
   constexpr int kAhead = 2;
   const T* c = reinterpret_cast<const T*>(p.c) + m * p.ldc_m + n;
   for (int k0 = 0; k0 < p.top_k; k0 += kAhead) {
-    Word v[kAhead];
+    Word v[kAhead][GROUPS];
     bool on[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int k = k0 + i;
       on[i] = k < p.top_k && !(p.ids && unsigned(__ldg(p.ids + m * p.top_k + k)) - unsigned(p.first) >= unsigned(p.E));
-      if (on[i]) v[i] = *reinterpret_cast<const Word*>(c + k * p.ldc_k);
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+        if (on[i] && there(g)) v[i][g] = *reinterpret_cast<const Word*>(c + k * p.ldc_k + g * 256 * VEC);
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (on[i]) add(v[i], p.w ? __ldg(p.w + m * p.top_k + k0 + i) : 1.f);
+    for (int i = 0; i < kAhead; ++i) {
+      if (!on[i]) continue;
+      const float w = p.w ? __ldg(p.w + m * p.top_k + k0 + i) : 1.f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+        if (there(g)) add(g, v[i][g], w);
+    }
   }
-  if (p.residual) add(*reinterpret_cast<const Word*>(reinterpret_cast<const T*>(p.residual) + m * p.ldr + n), 1.f);
   T* out = reinterpret_cast<T*>(p.out) + m * p.ldo + n;
-  if constexpr (VEC == 8)
-    *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[0], acc[1]), pack2<T>(acc[2], acc[3]), pack2<T>(acc[4], acc[5]), pack2<T>(acc[6], acc[7]));
-  else
-    *out = from_f32<T>(acc[0]);
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    if (!there(g)) continue;
+    if (p.residual) add(g, *reinterpret_cast<const Word*>(reinterpret_cast<const T*>(p.residual) + m * p.ldr + n + g * 256 * VEC), 1.f);
+    if constexpr (VEC == 8)
+      *reinterpret_cast<uint4*>(out) = make_uint4(pack2<T>(acc[g][0], acc[g][1]), pack2<T>(acc[g][2], acc[g][3]), pack2<T>(acc[g][4], acc[g][5]), pack2<T>(acc[g][6], acc[g][7]));
+    else if constexpr (VEC == 2)
+      *reinterpret_cast<uint32_t*>(out + g * 512) = pack2<T>(acc[g][0], acc[g][1]);
+    else
+      out[g * 256] = from_f32<T>(acc[g][0]);
+  }
 }
 
-template <typename T> int launch_combine(const CombineParams& p, cudaStream_t st) {
-  auto aligned = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % 8 == 0; };
-  const bool vec = p.N % 8 == 0 && aligned(p.c, p.ldc_m) && p.ldc_k % 8 == 0 && aligned(p.out, p.ldo) &&
-                   (!p.residual || aligned(p.residual, p.ldr));
-  const int per = 256 * (vec ? 8 : 1);
-  const int64_t chunks = (int64_t(p.N) + per - 1) / per;
+template <typename T, int VEC, int GROUPS> int launch_combine_as(const CombineParams& p, cudaStream_t st) {
+  const int64_t chunks = (int64_t(p.N) + 256 * VEC * GROUPS - 1) / (256 * VEC * GROUPS);
   if (chunks > 65535) return fail(FNN_ERR_UNSUPPORTED, "moe_combine: rows of %d columns are too long", p.N);
-  const dim3 grid(unsigned(p.M), unsigned(chunks));
-  if (vec) moe_combine_kernel<T, 8><<<grid, 256, 0, st>>>(p);
-  else moe_combine_kernel<T, 1><<<grid, 256, 0, st>>>(p);
+  moe_combine_kernel<T, VEC, GROUPS><<<dim3(unsigned(p.M), unsigned(chunks)), 256, 0, st>>>(p);
   return check_cuda(cudaGetLastError(), "moe_combine launch");
+}
+template <typename T> int launch_combine(const CombineParams& p, cudaStream_t st) {
+  // whether every access of `cols` columns is aligned
+  auto fits = [&](int cols) {
+    auto ok = [&](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % (cols * sizeof(T)) == 0 && ld % cols == 0; };
+    return p.N % cols == 0 && ok(p.c, p.ldc_m) && p.ldc_k % cols == 0 && ok(p.out, p.ldo) && (!p.residual || ok(p.residual, p.ldr));
+  };
+  if (fits(8)) return launch_combine_as<T, 8, 1>(p, st);
+  // Narrow accesses, two or four to a thread: four where the row is longer than two cover.  1 / 2 / 4 accesses, us: 4096 x 8 x
+  // 1001 53 / 35 / 27, x 4097 212 / 133 / 98, x 4098 (2 columns an access; 1 column in the first figure) 212 / 81 / 67;
+  // but 4096 x 8 x 1002 53 / 22 / 25, 16384 x 3 x 333 49 / 40 / 45.
+  if (fits(2)) return p.N > 2 * 256 * 2 ? launch_combine_as<T, 2, 4>(p, st) : launch_combine_as<T, 2, 2>(p, st);
+  return p.N > 2 * 256 ? launch_combine_as<T, 1, 4>(p, st) : launch_combine_as<T, 1, 2>(p, st);
 }
 
 }  // namespace

@@ -414,6 +414,27 @@ def test_combine_strides():
     assert torch.equal(flashnn_b200.moe_combine(c[:, :0]), torch.zeros(m, n, device="cuda").half())
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [2, 257, 511, 513, 1002, 1025, 1026, 2050, 2305])
+def test_combine_narrow_columns(n, dt):
+    """Rows of columns that no 16-byte access fits: each width of access and the rows' ends; nothing beside them is written."""
+    import flashnn_b200
+    m, k = 5, 3
+    g = _gen(n)
+    c = torch.randn(m, k, n, generator=g, device="cuda").to(dt)
+    w = torch.rand(m, k, generator=g, device="cuda")
+    r = torch.randn(m, n, generator=g, device="cuda").to(dt)
+    want = flashnn_b200.moe_combine(c, w, residual=r)
+    within(want, *O.combine(c, w, residual=r))
+    ids = torch.randint(0, 4, (m, k), generator=g, device="cuda", dtype=torch.int32)
+    d = c.clone()
+    d[ids >= 2] = float("nan")
+    within(flashnn_b200.moe_combine(d, w, ids, 2, residual=r), *O.combine(d, w, ids, 2, 0, r))
+    odd = torch.randn(m * k * n + 1, generator=g, device="cuda").to(dt)[1:].view(m, k, n)  # one element off every boundary
+    odd.copy_(c)
+    assert torch.equal(flashnn_b200.moe_combine(odd, w, residual=r), want)
+
+
 def test_combine_offsets_beyond_32_bits():
     import flashnn_b200
     m, k, n = 3, 2, 8192

@@ -25,15 +25,19 @@ def activate(v, name):
 
 def activation_error(v, y, name):
     """How far an fp32 evaluation at v may be off y = activate(v): the hardware exponential is within 2 + 1.173 |x| steps of
-    2^-23, reciprocal, sum and products within 6 more; where the sigmoid is below 2^-126 (|v| < 2^7) it may be taken as 0.
-    The erf is within 1.5e-7 < 2.6 * 2^-24, of which half goes into Phi, and 2.7 roundings of at most 1 follow."""
+    2^-23, reciprocal, sum and products within 6 more; where the sigmoid, also the one that gelu_tanh multiplies v by, is below 2^-126
+    (|v| < 2^7) it may be taken as 0.
+    GELU: v times a tail whose error is relative to itself: the exponential 4 roundings of 2^-24 and its argument at most 2 v^2, the
+    reciprocal 2 and its argument 1 (either weighs at most 1.7 in the tail), the fit 1.6, Horner's scheme and the products 6;
+    below 20 + 2 v^2 together.  Near 0, where half of that goes into Phi, an evaluation in 32 bits with the reciprocal one step
+    off either way is within 3.5 |v| roundings.  Where e^(-v^2 / 2) is below 2^-126 the result may be 0."""
     if name in ("sigmoid", "silu"):
         return y.abs() * 2 * U32 * (8 + 1.2 * v.abs()) + 2.0 ** -119
     if name == "gelu":
-        return v.abs() * 4 * U32
+        return torch.minimum(v.abs() * 4 * U32, y.abs() * U32 * (20 + 2 * v * v) + 2.0 ** -119)
     if name == "gelu_tanh":
         t = math.sqrt(8 / math.pi) * (v.abs() + 0.044715 * v.abs() ** 3)
-        return y.abs() * 2 * U32 * (8 + 4 * t)  # the argument's own four roundings included
+        return y.abs() * 2 * U32 * (8 + 4 * t) + 2.0 ** -119  # the argument's own four roundings included
     return torch.zeros_like(y)
 
 

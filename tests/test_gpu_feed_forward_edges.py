@@ -1,0 +1,29 @@
+"""The feed-forward operators where rounding, choice of kernel or sharing of memory shows: tails of the activations, zeros' signs,
+every tile width, runs of expert blocks, waits that run out, captured graphs side by side."""
+import pytest
+import torch
+
+from oracle import feed_forward as O
+from tests.test_gpu_feed_forward import DTYPES, gemm_case, run_gemm, within
+
+pytestmark = pytest.mark.gpu
+
+
+# streaming, cluster, single-CTA and CTA-pair kernel, and the generic one (no products)
+KERNELS = [(2, 512, 4096), (16, 200, 4096), (100, 2000, 256), (400, 1000, 512), (3, 40, 0)]
+
+
+@pytest.mark.parametrize("m,n,k", KERNELS)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu", "sigmoid"])
+def test_negative_tails_are_relatively_exact(act, m, n, k):
+    """The products are 0 and the bias is what the activation sees: the result is off by the output's half step and the few
+    roundings that the bound counts, relative to a value that falls to the smallest of the type."""
+    for out_ty in DTYPES:
+        for gated in (False, True):
+            c = gemm_case(m, n, k, gated, True, False, out_ty, bias_dt=torch.float32)
+            c["a"].zero_()
+            c["bias"][:n] = torch.linspace(-14, 1, n, device="cuda")
+            if gated:
+                c["bias"][n:] = 4096.0  # the other factor brings the tail back into fp16's normal range
+            v = c["bias"].double().expand(m, -1)  # (exactly what the activation sees: no error to carry through it)
+            within(run_gemm(c, act, gated, out_ty), *O.finish(v, torch.zeros_like(v), gated, act, None, out_ty))

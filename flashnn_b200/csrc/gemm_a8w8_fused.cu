@@ -169,6 +169,7 @@ a8w8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   }
 
   // a thread's outputs: four columns of a row at a time; what its first ones need from global memory is on its way during the barrier
+  // (an absent bias or residual is -0, which leaves every number as it is, a zero's sign included)
   struct Item {
     float rs, cs[4], bs[4], cu[4], bu[4], res[4];
   };
@@ -182,12 +183,12 @@ a8w8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     for (int j = 0; j < 4; ++j) {
       const bool on = col + j < p.N;
       t.cs[j] = on ? load_as_f32(p.alpha_col, p.col_dtype, col + j) : 0.f;
-      t.bs[j] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, col + j) : 0.f;
+      t.bs[j] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, col + j) : -0.f;
       if (FX::kGated) {
         t.cu[j] = on ? load_as_f32(p.alpha_col, p.col_dtype, int64_t(p.N) + col + j) : 0.f;
-        t.bu[j] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, int64_t(p.N) + col + j) : 0.f;
+        t.bu[j] = (on && fx.bias) ? load_as_f32(fx.bias, fx.bias_dtype, int64_t(p.N) + col + j) : -0.f;
       }
-      t.res[j] = (on && fx.residual) ? to_f32(reinterpret_cast<const OutT*>(fx.residual)[int64_t(row) * fx.ldr + col + j]) : 0.f;
+      t.res[j] = (on && fx.residual) ? to_f32(reinterpret_cast<const OutT*>(fx.residual)[int64_t(row) * fx.ldr + col + j]) : -0.f;
     }
   };
   int i = rank * kThreads + int(threadIdx.x);

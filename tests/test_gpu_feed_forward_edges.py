@@ -27,3 +27,26 @@ def test_negative_tails_are_relatively_exact(act, m, n, k):
                 c["bias"][n:] = 4096.0  # the other factor brings the tail back into fp16's normal range
             v = c["bias"].double().expand(m, -1)  # (exactly what the activation sees: no error to carry through it)
             within(run_gemm(c, act, gated, out_ty), *O.finish(v, torch.zeros_like(v), gated, act, None, out_ty))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [s for s in KERNELS if s[2]])
+def test_every_kernel_gives_the_generic_kernels_bits(m, n, k, gated):
+    """The choice of kernel does not show, not even in the sign of a zero: the generic kernel, which a misaligned operand takes,
+    computes one output at a time."""
+    for i, act in enumerate(O.ACTIVATIONS):
+        for j in range(4):
+            out_ty = DTYPES[(i + j) % 2]
+            c = gemm_case(m, n, k, gated, j & 1, j & 2, out_ty, seed=i)
+            c["a"][::2] = 0
+            c["row"][1] *= -1
+            c["col"][::3] *= -1
+            off = torch.zeros(m, k + 5, dtype=torch.int8, device="cuda")[:, 3:3 + k]
+            off.copy_(c["a"])
+            fast, generic = run_gemm(c, act, gated, out_ty), run_gemm(dict(c, a=off), act, gated, out_ty)
+            assert torch.equal(fast.view(torch.int16), generic.view(torch.int16)), (act, j)
+    c = gemm_case(m, n, k, gated, False, False, torch.float16)
+    c["a"].zero_()
+    c["col"].neg_()
+    out = run_gemm(c, None, gated, torch.float16)
+    assert (torch.signbit(out) == (not gated)).all()  # (gated: -0 times -0)

@@ -103,7 +103,7 @@ a8w8_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         if (leader) report(p.status, abort_flag, DEV_TIMEOUT_PRODUCER);
         break;
       }
-      if (leader) {
+      if (leader && !(i == p.skip_kb && rank == 0)) {  // (test hook: one K block's loads left out)
         uint8_t* sa = smem + stage * L::kStageBytes;
         mbar_expect_tx(&full_bar[stage], L::kStageBytes);
         tma_load_2d(sa + L::kABytes, &tmap_b, &full_bar[stage], kb * kBK, n0);
@@ -267,6 +267,10 @@ int launch_split(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, A8W
   if (int e = make_tmap_i8(&tb, b, fx.rows, p.K, ldb, OW)) return e;
   p.tiles_n = (p.N + OW - 1) / OW;
   p.k_blocks = (p.K + kBK - 1) / kBK;
+  if (const int stall_us = opt_test_stall_us()) {  // test hook: make one wait of every cluster's first CTA run out quickly
+    p.wait_ns = 1000ull * unsigned(stall_us);
+    p.skip_kb = 1;  // (a CTA has four K blocks or more)
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(p.tiles_n * splits));
   cfg.blockDim = dim3(kThreads);

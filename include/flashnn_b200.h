@@ -80,6 +80,8 @@ typedef enum fnn_moe_group_score { FNN_GROUP_MAX = 0, FNN_GROUP_TOP2 = 1 } fnn_m
  * seconds.  The wait for the missing block then runs out: the kernel records its time-out code, drains what it has in
  * flight, frees what it holds and returns without a result, and the next fnn_device_status reports
  * FNN_ERR_DEVICE_TIMEOUT.  This is how the give-up path of the kernels is exercised without faulting the GPU.
+ * fnn_gemm_a8w8_epilogue obeys it in the same kernel and in the one whose clusters share the K blocks of a tile (up to 128 rows, few
+ * tiles, long K), there in the first CTA of every cluster; what such a launch leaves in its output is undefined.
  *
  * FNN_OPT_A8W8_PAIR_TILE (default 0 = chosen from the problem shape; a tuning hook).  128, 160, 192, 224 or 256 forces
  * that output-tile width in fnn_gemm_a8w8 wherever the CTA-pair tensor-core kernel can run (more than 128 rows).  The

@@ -1,10 +1,13 @@
 """The feed-forward operators where rounding, choice of kernel or sharing of memory shows: tails of the activations, zeros' signs,
 every tile width, runs of expert blocks, waits that run out, captured graphs side by side."""
+import ctypes
+import time
+
 import pytest
 import torch
 
 from oracle import feed_forward as O
-from tests.test_gpu_feed_forward import DTYPES, gemm_case, run_gemm, within
+from tests.test_gpu_feed_forward import DTYPES, check_gemm, gemm_case, run_gemm, within
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +53,29 @@ def test_every_kernel_gives_the_generic_kernels_bits(m, n, k, gated):
     c["col"].neg_()
     out = run_gemm(c, None, gated, torch.float16)
     assert (torch.signbit(out) == (not gated)).all()  # (gated: -0 times -0)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# waits that run out
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", [(16, 200, 4096), (64, 130, 4112), (128, 200, 28672)])
+def test_a_wait_of_the_cluster_kernel_runs_out(m, n, k, gated):
+    """A test option shortens the waits of one launch and leaves out the loads of one K block in the first CTA of every cluster.  The
+    launch ends, the host reads the status once, and the same call then gives the same right answer as before."""
+    from flashnn_b200 import _lib
+    L = _lib.lib()
+    c = gemm_case(m, n, k, gated, True, True, torch.bfloat16, seed=n)
+    want = check_gemm(c, "silu", gated, torch.bfloat16)
+    _lib.set_option(_lib.OPT_TEST_STALL_US, 20000)
+    try:
+        start = time.perf_counter()
+        with pytest.raises(_lib.FlashNNError) as err:
+            run_gemm(c, "silu", gated, torch.bfloat16)  # (reads the device status after its call)
+        assert time.perf_counter() - start < 2.0
+    finally:
+        _lib.set_option(_lib.OPT_TEST_STALL_US, 0)
+    assert err.value.status == 8 and "bounded wait" in err.value.message
+    code = ctypes.c_int(0)
+    assert L.fnn_device_status(ctypes.byref(code)) == 0 and code.value == 0
+    assert torch.equal(check_gemm(c, "silu", gated, torch.bfloat16), want)

@@ -13,13 +13,17 @@ from .kernel_backend import BackendKernel
 
 _DT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
-# scratch per (device, stream): weight-only zero-point path.  Work on one stream is ordered, so one buffer per stream
-# is enough; the least recently used entries are dropped beyond a handful of streams.
+# scratch per (device, stream) of the products that need some.  Work on one stream is ordered, so one buffer per stream is
+# enough; the least recently used entries are dropped beyond a handful of streams.  A call that is being captured gets a
+# buffer of its own from the graph's memory: graphs captured on one stream can be replayed side by side, and a graph
+# outlives what this dictionary drops or replaces.
 _workspaces = collections.OrderedDict()
 _MAX_WORKSPACES = 8
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:

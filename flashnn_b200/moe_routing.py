@@ -21,8 +21,11 @@ class MoeRouting(BackendKernel):
     equal ones by the lowest index; their weights are the scores (without the bias), divided by their sum if `renormalize`,
     times `scale`.  With num_groups > 1 only the experts of the best `topk_groups` groups of E / num_groups consecutive ones
     can be chosen; a group's score is the largest score + bias in it ("max") or the sum of its two largest ("top2").
-    The order is that of 64-bit arithmetic.  A logit of -inf takes an expert out (under the sigmoid with a bias: a bias of
-    -inf), while top_k others are left."""
+    The order is that of 64-bit arithmetic; the bias is taken in fp32.
+
+    Taking an expert out: without a bias by a logit of -inf; with one by a bias of -inf, under either scoring.  With a bias a logit of
+    -inf only makes the score 0: the expert still competes with bias[e], ahead of live experts whose score + bias is below that,
+    and has the weight 0 if it wins.  An expert that is out is chosen only where fewer than top_k others can be."""
 
     def __init__(self, num_experts: int, top_k: int, scoring: str = "softmax", renormalize: bool = True, num_groups: int = 1,
                  topk_groups: int = 1, group_score: str = "max", scale: float = 1.0):

@@ -275,7 +275,8 @@ int fnn_fused_moe_a8w8_gated(const int8_t* a, int64_t lda, const int8_t* b, int6
  *     ids      the top_k experts with the largest keys among them, in that order
  *     weights  score[ids], divided by their sum if renormalize, times scale
  * The order is that of 64-bit arithmetic, equal keys go to the lowest index.  A NaN key ranks last, with the -infinities.  A
- * row of -infinity logits has the weights 0 under the softmax.
+ * row of -infinity logits has the weights 0 under the softmax.  A logit of -infinity is a score of 0: it takes an expert out
+ * where there is no bias; with one the expert's key is its bias, and a bias of -infinity takes it out.
  *
  *   logits        [M, E]  f16, bf16 or f32, ldl;  E at most 1024
  *   bias          NULL or [E] f32

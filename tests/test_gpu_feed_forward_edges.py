@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import feed_forward as O
-from tests.test_gpu_feed_forward import DTYPES, check_gemm, gemm_case, run_gemm, within
+from tests.test_gpu_feed_forward import DTYPES, check_gemm, check_route, gemm_case, run_gemm, within
 
 pytestmark = pytest.mark.gpu
 
@@ -53,6 +53,35 @@ def test_every_kernel_gives_the_generic_kernels_bits(m, n, k, gated):
     c["col"].neg_()
     out = run_gemm(c, None, gated, torch.float16)
     assert (torch.signbit(out) == (not gated)).all()  # (gated: -0 times -0)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# routing
+# ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups,tg", [(24, 1, 1), (24, 3, 2), (96, 1, 1), (96, 8, 3), (448, 8, 5)])
+def test_masked_experts_and_a_bias_that_is_not_zero(e, groups, tg, scoring):
+    """A logit of -inf leaves an expert its bias, a bias of -inf takes it out: single experts, a group, all but a few."""
+    g = torch.Generator(device="cuda").manual_seed(e)
+    x = torch.randn(60, e, generator=g, device="cuda")
+    out = torch.zeros(e, dtype=torch.bool, device="cuda")
+    out[torch.randperm(e, generator=g, device="cuda")[: e // 5]] = True
+    x[:20, out] = -float("inf")
+    x[20:30, : e // max(groups, 2)] = -float("inf")
+    x[30:33, 3:] = -float("inf")
+    for gs in ("max", "top2") if groups > 1 else ("max",):
+        kw = dict(scoring=scoring, num_groups=groups, topk_groups=tg, group_score=gs)
+        for lo, hi in ((-0.5, 0.5), (0.0, 0.2), (-0.2, 0.0)):
+            bias = torch.rand(e, generator=g, device="cuda") * (hi - lo) + lo
+            check_route(x, 5, bias, **kw)
+            bias[out] = -float("inf")
+            _, ids = check_route(x[33:], 5, bias, **kw)
+            assert not out[ids.long()].any()
+            check_route(x, 5, bias, **kw)
+            bias[: e // max(groups, 2)] = -float("inf")
+            check_route(x, 5, bias, **kw)
+            bias[2:] = -float("inf")
+            check_route(x, 5, bias, **kw)
 
 
 # ---------------------------------------------------------------------------------------------------------------

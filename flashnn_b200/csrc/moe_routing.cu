@@ -1093,7 +1093,9 @@ extern "C" int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_
   if (num_choices < 0 || E <= 0 || block_m <= 0 || EM < 0)
     return fail(FNN_ERR_SHAPE, "moe_sort: num_choices=%lld E=%lld block_m=%d EM=%lld", (long long)num_choices, (long long)E, block_m, (long long)EM);
   if (E > kSortMaxExperts) return fail(FNN_ERR_UNSUPPORTED, "moe_sort: at most %d experts (got %lld)", kSortMaxExperts, (long long)E);
-  if (first_expert < INT32_MIN || first_expert > INT32_MAX) return fail(FNN_ERR_SHAPE, "moe_sort: first_expert must fit 32 bits");
+  // (the kernel compares unsigned differences: a range that passes 2^31 would take in the numbers it wraps to)
+  if (first_expert < INT32_MIN || first_expert > INT32_MAX || first_expert + E > int64_t(INT32_MAX) + 1)
+    return fail(FNN_ERR_SHAPE, "moe_sort: expert numbers must fit 32 bits");
   const int64_t need = fnn_moe_sort_slots(num_choices, E, block_m);
   if (num_choices > INT32_MAX / 2 || need > INT32_MAX / 2) return fail(FNN_ERR_SHAPE, "moe_sort: %lld choices need %lld slots: too many", (long long)num_choices, (long long)need);
   if (EM != need) return fail(FNN_ERR_SHAPE, "moe_sort: the slot list has %lld entries, fnn_moe_sort_slots says %lld", (long long)EM, (long long)need);
@@ -1151,8 +1153,8 @@ extern "C" int fnn_moe_combine(const void* c, int dtype, int64_t ldc_m, int64_t 
     return fail(FNN_ERR_SHAPE, "moe_combine: M=%lld top_k=%lld N=%lld ldc_m=%lld ldc_k=%lld ldr=%lld ldo=%lld E=%lld", (long long)M,
                 (long long)top_k, (long long)N, (long long)ldc_m, (long long)ldc_k, (long long)ldr, (long long)ldo, (long long)E);
   if (M > INT32_MAX || N > INT32_MAX || top_k > INT32_MAX) return fail(FNN_ERR_SHAPE, "moe_combine: sizes must be below 2^31");
-  if (topk_ids && (E > INT32_MAX || first_expert < INT32_MIN || first_expert > INT32_MAX))
-    return fail(FNN_ERR_SHAPE, "moe_combine: E and first_expert must fit 32 bits");
+  if (topk_ids && (E > INT32_MAX || first_expert < INT32_MIN || first_expert > INT32_MAX || first_expert + E > int64_t(INT32_MAX) + 1))
+    return fail(FNN_ERR_SHAPE, "moe_combine: expert numbers must fit 32 bits");
   if (dtype != FNN_F16 && dtype != FNN_BF16) return fail(FNN_ERR_DTYPE, "moe_combine: the expert outputs must be f16 or bf16 (got dtype code %d)", dtype);
   if (M == 0 || N == 0) return FNN_OK;
   if (!out || (top_k > 0 && !c)) return fail(FNN_ERR_NULL_POINTER, "moe_combine: null tensor pointer");

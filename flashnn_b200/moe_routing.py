@@ -78,6 +78,7 @@ def moe_sort_tokens(topk_ids, num_experts, BM, first_expert=0):
     assert topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64"
     assert num_experts >= 1 and BM >= 1, "num_experts and BM must be positive"
     assert first_expert >= 0, "first_expert must not be negative"
+    assert first_expert + num_experts < 2 ** 31, "expert numbers must be below 2^31 - 1"  # (64-bit ones are cut off there)
     ids = _ids32(topk_ids)
     if not ids.is_contiguous():
         ids = ids.contiguous()
@@ -120,6 +121,7 @@ def moe_combine(C, topk_weights=None, topk_ids=None, num_experts=None, first_exp
         assert topk_ids.shape == (m, k) and num_experts is not None and num_experts >= 1, "topk_ids must be [M, top_k], with num_experts"
         assert topk_ids.dtype in (torch.int32, torch.int64), "topk_ids must be int32 or int64"
         assert first_expert >= 0, "first_expert must not be negative"
+        assert first_expert + num_experts < 2 ** 31, "expert numbers must be below 2^31 - 1"
         topk_ids, experts = _ids32(topk_ids), num_experts
         if not topk_ids.is_contiguous():
             topk_ids = topk_ids.contiguous()

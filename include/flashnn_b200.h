@@ -296,7 +296,7 @@ int fnn_moe_route(const void* logits, int logits_dtype, int64_t ldl, int64_t M, 
  *   topk_ids          [num_choices] int32
  *   sorted_token_ids  [EM] int32, EM = fnn_moe_sort_slots(num_choices, E, block_m): the most that any choice of experts fills
  *   expert_ids        [EM / block_m] int32;  num_tokens_post_padded [1] int32 (device memory): slots in use
- *   E                 at most 1024
+ *   E                 at most 1024; first_expert + E at most 2^31
  */
 int fnn_moe_sort(const int32_t* topk_ids, int64_t num_choices, int64_t E, int64_t first_expert, int block_m,
                  int32_t* sorted_token_ids, int64_t EM, int32_t* expert_ids, int32_t* num_tokens_post_padded, void* stream);
@@ -309,7 +309,7 @@ int64_t fnn_moe_sort_slots(int64_t num_choices, int64_t E, int block_m);
  *   c             [M, top_k, N] f16 or bf16 (dtype), ldc_m and ldc_k elements between tokens and between choices
  *   topk_weights  NULL (all 1, the expert products have applied them) or [M, top_k] f32, contiguous
  *   topk_ids      NULL or [M, top_k] int32, contiguous: choices of experts outside [first_expert, first_expert + E) are left out,
- *                 and their rows of c, which nothing has written, are not read
+ *                 and their rows of c, which nothing has written, are not read; first_expert + E at most 2^31
  *   residual      NULL or [M, N] in dtype, ldr (0: the same row for every m);  it may be `out` itself (same pointer, ldr == ldo)
  *   out           [M, N] in dtype, ldo
  */

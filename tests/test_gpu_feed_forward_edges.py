@@ -84,6 +84,21 @@ def test_masked_experts_and_a_bias_that_is_not_zero(e, groups, tg, scoring):
             check_route(x, 5, bias, **kw)
 
 
+def test_experts_up_to_the_largest_number():
+    import flashnn_b200 as F
+    top = 2 ** 31 - 1
+    ids = torch.tensor([[top - 1, -2 ** 31], [top, top - 2], [-1, 0]], device="cuda")
+    for x in (ids, ids.int(), torch.where(ids == top, 2 ** 40, ids)):  # 2^31 - 1 and all above are no expert
+        slots, experts, used = F.moe_sort_tokens(x, 2, 2, first_expert=top - 2)
+        assert used.tolist() == [4] and slots[:4].tolist() == [3, 6, 0, 6] and experts[:2].tolist() == [0, 1]
+        c = torch.arange(1, 7, device="cuda").half().view(3, 2, 1)
+        assert F.moe_combine(c, topk_ids=x, num_experts=2, first_expert=top - 2).flatten().tolist() == [1, 4, 0]
+        for call in (lambda: F.moe_sort_tokens(x, 3, 2, first_expert=top - 2),
+                     lambda: F.moe_combine(c, topk_ids=x, num_experts=3, first_expert=top - 2)):
+            with pytest.raises(AssertionError, match="2\\^31"):
+                call()
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # waits that run out
 # ---------------------------------------------------------------------------------------------------------------

@@ -56,7 +56,10 @@ def fused_moe_a8w8_gated_forward(A, B, C, alpha_row_ptr, alpha_col_ptr, topk_ids
     A [M, K] int8; B [E, 2 N, K] int8: an expert's N rows inside the activation, then the N rows that its value
     multiplies; C [M, top_k, N] fp16/bf16 (written in place, rows named by no slot are left alone); alpha_row_ptr [M];
     alpha_col_ptr [E, 2 N]; bias None or [E, 2 N]; sorted_token_ids [EM], expert_ids [EM / BM] and num_tokens_post_padded [1]
-    as `moe_sort_tokens` gives them; activation "none", "relu", "sigmoid", "silu", "gelu" or "gelu_tanh"."""
+    as `moe_sort_tokens` gives them; activation "none", "relu", "sigmoid", "silu", "gelu" or "gelu_tanh".
+
+    BM: 16 for few tokens per expert, 256 for hundreds.  More than 1024 blocks of less than 128 slots are slow: an expert's weights are
+    then read again for each of its blocks."""
     index = _one_device(A, B, C, alpha_row_ptr, alpha_col_ptr, bias, sorted_token_ids, expert_ids, num_tokens_post_padded)
     act = _lib.ACTIVATIONS.get(activation)
     assert act is not None, f"unknown activation {activation!r}"

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import feed_forward as O
-from tests.test_gpu_feed_forward import DTYPES, check_gemm, check_route, gemm_case, run_gemm, within
+from tests.test_gpu_feed_forward import DTYPES, check_experts, check_gemm, check_route, experts_case, gemm_case, run_gemm, within
 
 pytestmark = pytest.mark.gpu
 
@@ -55,6 +55,19 @@ def test_every_kernel_gives_the_generic_kernels_bits(m, n, k, gated):
     assert (torch.signbit(out) == (not gated)).all()  # (gated: -0 times -0)
 
 
+@pytest.mark.parametrize("k", [128, 2304])  # with 16 and with 8 epilogue warps
+def test_all_widths_of_the_pair_tile(k):
+    """Every width that the plan can choose, by name: five without a gate, three with one (half a tile is whole chunks of 32 columns;
+    where the plan for the accumulator columns takes one of the three, the gated plan takes it too)."""
+    from flashnn_b200 import _lib
+    for gated, widths, shapes in ((False, (128, 160, 192, 224, 256), [(136, 4744), (136, 9480), (136, 11848), (257, 7112), (257, 8296)]),
+                                  (True, (128, 192, 256), [(136, 2372), (136, 5924), (257, 4148)])):
+        for width, (m, n) in zip(widths, shapes):
+            assert _lib.a8w8_plan(m, 2 * n if gated else n, k) == (1, width)
+            for i, out_ty in enumerate(DTYPES):
+                check_gemm(gemm_case(m, n - i, k, gated, True, not i, out_ty, seed=width), "silu" if i else "gelu", gated, out_ty)
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # routing
 # ---------------------------------------------------------------------------------------------------------------
@@ -97,6 +110,29 @@ def test_experts_up_to_the_largest_number():
                      lambda: F.moe_combine(c, topk_ids=x, num_experts=3, first_expert=top - 2)):
             with pytest.raises(AssertionError, match="2\\^31"):
                 call()
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# gated expert products: runs of an expert's blocks
+# ---------------------------------------------------------------------------------------------------------------
+# By the rule of the launch, on 148 SMs: a mean of up to 48 choices per expert and blocks of up to 32 slots make runs of up to 64 rows, else
+# 128; the widest of 256, 128 and 64 accumulator columns that gives every SM a tile.  n: 2500 -> 256, 1300 -> 128, 300 -> 64.
+@pytest.mark.parametrize("n", [2500, 1300, 301])
+@pytest.mark.parametrize("m,bm", [(64, 16), (150, 32), (40, 5), (512, 16), (700, 64), (600, 48), (257, 32)])
+def test_runs_of_every_height_and_width(m, bm, n):
+    for i, out_ty in enumerate(DTYPES):
+        c = experts_case(m, 8, n, 144, 2, not i, out_ty, seed=m + n, dropped=0.1 * i)
+        if i:
+            c["ids"][: m // 2] = 6  # more than half of the choices are one expert's, so that it has several runs
+        check_experts(c, "silu", bm, out_ty)
+
+
+@pytest.mark.parametrize("m,blocks", [(8132, 1024), (8140, 1025), (20000, 2507)])
+def test_slot_lists_around_the_longest_that_is_gathered_into_runs(m, blocks):
+    """Up to 1024 blocks are gathered into runs; a longer list has a tile for every block."""
+    from flashnn_b200 import _lib
+    assert _lib.lib().fnn_moe_sort_slots(2 * m, 8, 16) == 16 * blocks
+    check_experts(experts_case(m, 8, 70, 80, 2, True, torch.bfloat16, seed=m, dropped=0.1), "silu", 16, torch.bfloat16)
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -331,9 +331,10 @@ int dispatch_fused(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, c
   }
   const A8W8Plan plan = plan_a8w8(p.M, p.N, sm_count(), FX::kGated);
   // With K up to 2048 a tile waits for its epilogue, and 16 warps finish it sooner than 8 (two against four per scheduler, chunks of
-  // 16 columns): 4096 x 8192 x 1024, none 38 -> 34 us, silu 53 -> 48, bias + gelu + residual 79 -> 73; at 2048 silu 57 -> 53; from 4096 on
-  // the MMAs hide either, and the expert products, which scatter rows, take 5 % longer with 16.  What then bounds the epilogue is the
-  // pipe of the conversions, exponentials and reciprocals: three of its slots an element with silu.
+  // 16 columns): 4096 x 8192 x 1024, none 38 -> 34 us, silu 53 -> 48, bias + gelu + residual 79 -> 73 (66 with the present gelu); at 2048
+  // silu 57 -> 53; from 4096 on the MMAs hide either, and the expert products, which scatter rows, take 5 % longer with 16.  No pipe
+  // bounds what is left: with silu at K = 1024 the tensor pipe is busy 37 % of the time and that of conversions, exponentials and
+  // reciprocals (three slots an element) 39 %; the warps wait for one another's results and for TMEM.
   if (plan.pair) return p.K <= 2048 ? launch_pair_width<OutT, 16>(plan.bn, a, lda, b, ldb, p, fx, st) : launch_pair_width<OutT, 8>(plan.bn, a, lda, b, ldb, p, fx, st);
   if (plan.bn == 256) return launch_umma_rows<OutT, 256>(a, lda, b, ldb, p, st, fx);
   if (plan.bn == 128) return launch_umma_rows<OutT, 128>(a, lda, b, ldb, p, st, fx);

@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(WARPS * 32, 24 / WARPS) moe_route_kernel(const
 // need no expert numbers: a lane sorts its keys eight (or 16) at a time and merges them into its eight largest, a butterfly merges the lanes',
 // and the top_k-th of the result is all that is kept.  The keys that are not below it, less the tolerance, are the candidates,
 // top_k of them and rarely more; in a list, in expert order, each counts those before it, and that is its place.
-// 16384 tokens x 256 experts in groups, fp32 logits: one warp per token 980 instructions a row and 28 us, this kernel 430 and 17 us.
+// 16384 tokens x 256 experts in groups, fp32 logits: one warp per token 980 instructions a row and 28 us, this kernel 460 and 17 us.
 // Where fp32 does not decide, the two comparisons that can be in doubt (between groups, between candidates) are made in 64
 // bits here, in little code: the whole row in 64 bits costs a launch 8 us, most of it fetching instructions that no other row has run.
 // A row with more candidates than the list holds, or too few keys above -infinity, goes to the general form.

@@ -58,7 +58,7 @@ def fused_moe_a8w8_gated_forward(A, B, C, alpha_row_ptr, alpha_col_ptr, topk_ids
     alpha_col_ptr [E, 2 N]; bias None or [E, 2 N]; sorted_token_ids [EM], expert_ids [EM / BM] and num_tokens_post_padded [1]
     as `moe_sort_tokens` gives them; activation "none", "relu", "sigmoid", "silu", "gelu" or "gelu_tanh".
 
-    BM: 16 for few tokens per expert, 256 for hundreds.  More than 1024 blocks of less than 128 slots are slow: an expert's weights are
+    BM: 16 for few tokens per expert, 256 for hundreds.  More than 1024 blocks of up to 64 slots are slow: an expert's weights are
     then read again for each of its blocks."""
     index = _one_device(A, B, C, alpha_row_ptr, alpha_col_ptr, bias, sorted_token_ids, expert_ids, num_tokens_post_padded)
     act = _lib.ACTIVATIONS.get(activation)

@@ -77,3 +77,34 @@ def test_two_graphs_of_calls_with_workspaces_replay_side_by_side():
             for t in out:
                 t.zero_()
     assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_a_captured_hand_over_of_partial_sums_in_memory_that_the_graph_reuses():
+    """The product whose CTA pairs hand partial sums over keeps flags in its workspace, which needs no initialisation: replayed alone,
+    with other tensors in the same memory between its two calls and behind them."""
+    import flashnn_b200 as F
+    from flashnn_b200 import _lib
+    m, n, k = 4096, 2048, 16384
+    need = _lib.lib().fnn_gemm_a8w8_workspace_bytes(m, n, k)
+    assert need > 0
+    g = torch.Generator(device="cuda").manual_seed(0)
+    a, b = (torch.randint(-127, 128, (r, k), generator=g, device="cuda", dtype=torch.int8) for r in (m, n))
+    row, col = torch.rand(m, generator=g, device="cuda") * 0.01, torch.rand(n, generator=g, device="cuda") * 0.001
+    f = F.GemmA8W8(torch.bfloat16)
+    want = [f(a, b, row, col).clone(), f(a.flip(0), b, row, col).clone()]
+    rev = a.flip(0).contiguous()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = f(a, b, row, col)
+        torch.ones(need // 8, dtype=torch.int64, device="cuda")
+        second = f(rev, b, row, col)
+        torch.full((need // 8,), -1, dtype=torch.int64, device="cuda")
+    for _ in range(4):
+        first.zero_()
+        second.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want[0]) and torch.equal(second, want[1])
+    assert _lib.device_status() == 0
